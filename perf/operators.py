@@ -235,7 +235,7 @@ def _prepare_attention(case, seed):
     return {"case": case, "q": q, "cache": cache, "block_tables": _ints(tables), "cu_q": _ints(np.concatenate([[0], np.cumsum(q_lens)])),
             "context_lens": _ints(context), "tok_seq": _ints(np.repeat(np.arange(len(q_lens)), q_lens)),
             "positions": _ints(np.concatenate([c + np.arange(k) for c, k in zip(context, q_lens)])),
-            "shared_first": _ints(first), "shared_lens": _ints(shared), "n_tokens": n, "max_q_len": int(q_lens.max()),
+            "shared_first": _ints(first), "shared_lens": _ints(prefix_of), "n_tokens": n, "max_q_len": int(q_lens.max()),
             "max_shared_len": int(shared.max()), "max_own_len": int((before + q_lens).max()),
             "max_group_tokens": int(np.add.reduceat(q_lens, first[:-1]).max()), "status": _ints([0])}
 
@@ -347,7 +347,7 @@ def _plain_attention(s):
     """Scores of every group's tokens on its prefix and of every request's tokens on its own keys, one softmax over both."""
     c = s["case"]
     heads, kv_heads, dim, page = c["heads"], c["kv_heads"], c["dim"], c["page"]
-    n, n_seq, n_group, per = s["n_tokens"], s["context_lens"].numel(), s["shared_lens"].numel(), heads // kv_heads
+    n, n_seq, n_group, per = s["n_tokens"], s["context_lens"].numel(), s["shared_first"].numel() - 1, heads // kv_heads
     first, shared = s["shared_first"].long(), s["shared_lens"].long()
     seq, position = s["tok_seq"].long(), s["positions"].long()
     cu = s["cu_q"].long()
@@ -373,13 +373,13 @@ def _plain_attention(s):
     n_shared, n_own = -(-s["max_shared_len"] // page), -(-s["max_own_len"] // page) + 1
     zero = torch.zeros(n_group, dtype=torch.int64, device=seq.device)
     pk, pv = _pages_of(s, s["block_tables"][first[:-1]], zero, n_shared)
-    ok, ov = _pages_of(s, s["block_tables"], shared[group_of] // page, n_own)
+    ok, ov = _pages_of(s, s["block_tables"], shared // page, n_own)
     most_group, most_q = s["max_group_tokens"], s["max_q_len"]
     on_prefix = back(scores(n_group, in_group, group, most_group, pk), in_group, group, most_group)
     on_own = back(scores(n_seq, in_seq, seq, most_q, ok), in_seq, seq, most_q)
     kp = torch.arange(n_shared * page, device=seq.device)
-    ko = torch.arange(n_own * page, device=seq.device) + shared[group][:, None]
-    see_prefix = (kp < shared[group][:, None]) & (kp >= low[:, None])
+    ko = torch.arange(n_own * page, device=seq.device) + shared[seq][:, None]
+    see_prefix = (kp < shared[seq][:, None]) & (kp >= low[:, None])
     see_own = (ko <= position[:, None]) & (ko >= low[:, None])
     both = torch.cat([on_prefix.masked_fill(~see_prefix[:, None, None], -math.inf),
                       on_own.masked_fill(~see_own[:, None, None], -math.inf)], -1)
