@@ -40,6 +40,7 @@
 #include <math.h>
 
 #include "common.cuh"
+#include "shared_prefix.cuh"
 
 namespace {
 
@@ -75,7 +76,13 @@ struct MmaAttnParams {
     const float* sink;           // [heads] or null: exp(sink[h]) joins the softmax's denominator, with no value
     const float* distance;       // [2][heads] (r1, then r2) or null: scores lose r1 ln(1 + r2 (p - j))
     int beside;                  // the next kernel runs beside this one and takes what this one waited for (attention_tc.cu)
+    SharedPrefixParams shared;   // OWN_KEYS and SHARED_KEYS only
+    int part;                    // ... and the first of the parts that are written
 };
+
+// Which keys a launch covers. OWN_KEYS: those of a sequence from shared.lens[sequence] on; SHARED_KEYS (wide tiles): those
+// below it, for tiles of a group's tokens, read through the group's first sequence (attention_shared.cu). Both write parts.
+enum Keys { ALL_KEYS, OWN_KEYS, SHARED_KEYS };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2,
                                          unsigned a3, unsigned b0, unsigned b1) {
@@ -234,7 +241,7 @@ __device__ __forceinline__ void issue_chunk_warp(const MmaAttnParams& p, __nv_bf
 struct One { static constexpr int value = 1; };
 struct Two { static constexpr int value = 2; };
 
-template <int HD, bool NARROW, bool BIASED>
+template <int HD, bool NARROW, bool BIASED, Keys KEYS>
 __global__ void __launch_bounds__(NARROW ? NARROW_THREADS : MMA_THREADS, NARROW ? 1 : 3)
 attention_mma_kernel(const MmaAttnParams p) {
     constexpr int KB = HD / 32;                 // 32-wide blocks of the head dim
@@ -247,12 +254,28 @@ attention_mma_kernel(const MmaAttnParams p) {
     __shared__ __align__(8) unsigned long long bars[N_STAGES];
     __shared__ int narrow_table[NARROW ? NARROW_TABLE : 1];   // the sequence's first block-table entries
 
+    if (KEYS == SHARED_KEYS) pdl_wait();
     if (!p.beside) pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
     const int tile = blockIdx.x, kh = blockIdx.y, split = blockIdx.z;
     // no tile list: tile i is the whole of sequence i (a batch of decoding requests), one look-up less
-    const int seq = p.tiles ? p.tiles[2 * tile] : tile, tile_row0 = p.tiles ? p.tiles[2 * tile + 1] : 0;
+    int seq, tile_row0, q_start, q_len, ctx = 0;
+    if (KEYS == SHARED_KEYS) {
+        const GroupTile found = find_group_tile(p.shared, p.cu_q, tile, TILE_ROWS, p.group, lane);
+        if (found.tokens <= 0) return;
+        seq = found.seq; tile_row0 = found.first; q_start = found.q_start; q_len = found.tokens;
+    } else if (KEYS == OWN_KEYS && !NARROW) {
+        const SequenceTile found = find_sequence_tile(p.cu_q, p.shared.n_seqs, tile, TILE_ROWS, p.group, lane);
+        if (found.seq < 0) {
+            pdl_wait();
+            return;
+        }
+        seq = found.seq; tile_row0 = found.row;
+    } else {
+        seq = p.tiles ? p.tiles[2 * tile] : tile;
+        tile_row0 = p.tiles ? p.tiles[2 * tile + 1] : 0;
+    }
     if (NARROW) {
         // the block-table row sets out together with the sequence's lengths (it does not depend on
         // them): one trip to memory instead of two before the first page can be asked for
@@ -260,14 +283,19 @@ attention_mma_kernel(const MmaAttnParams p) {
         for (int e = threadIdx.x; e < min(p.bt_stride, NARROW_TABLE); e += blockDim.x) narrow_table[e] = row[e];
     }
     const int group = p.group;
-    const int q_start = p.cu_q[seq];
-    const int q_len = p.cu_q[seq + 1] - q_start;
-    const int ctx = p.context_lens[seq];
+    if (KEYS != SHARED_KEYS) {
+        q_start = p.cu_q[seq];
+        q_len = p.cu_q[seq + 1] - q_start;
+        ctx = p.context_lens[seq];
+    }
+    const int own_from = KEYS == OWN_KEYS && p.shared.lens != nullptr ? p.shared.lens[seq] : 0;
     const int n_rows = q_len * group;
     if (tile_row0 >= n_rows) {                  // a padding sequence of a fixed-size batch
-        if (p.beside) pdl_wait();               // a block that ends has let the next kernel start
+        if (p.beside || KEYS == OWN_KEYS) pdl_wait();   // a block that ends has let the next kernel start
         return;
     }
+    if (KEYS == OWN_KEYS && NARROW && n_rows > TILE_ROWS && tid == 0)
+        atomicOr(p.status, MX_STATUS_BAD_STEP);  // the sequence brings more tokens than the caller said any does
 
     if (tid == 0) {
 #pragma unroll
@@ -295,7 +323,12 @@ attention_mma_kernel(const MmaAttnParams p) {
         r_tok[i] = token_of(rr);
         r_head[i] = rr - r_tok[i] * group;
         r_pos[i] = ctx + r_tok[i];
-        r_lo[i] = first_visible_key(r_pos[i], p.window);
+        r_lo[i] = max(first_visible_key(r_pos[i], p.window), own_from);
+        if (KEYS == SHARED_KEYS) {
+            const KeyRange range = shared_keys_of_token(p.shared, q_start + r_tok[i], p.window);
+            r_pos[i] = range.last;
+            r_lo[i] = range.first;
+        }
     }
     float r1[2] = {0.f, 0.f}, r2[2] = {0.f, 0.f};    // distance bias of the row's head, in log2 units as it stands
     if (BIASED) {
@@ -306,20 +339,31 @@ attention_mma_kernel(const MmaAttnParams p) {
         }
     }
     // key range of the block (what is fetched) and of the warp (what it computes)
-    const int hi_tile = ctx + token_of(tile_last);
-    const int lo_tile = first_visible_key(ctx + token_of(tile_row0), p.window);
-    const int hi_warp = warp_has_rows ? ctx + token_of(last_row) : -1;
-    const int lo_warp = first_visible_key(ctx + token_of(row0), p.window);
+    int hi_tile = ctx + token_of(tile_last);
+    int lo_tile = max(first_visible_key(ctx + token_of(tile_row0), p.window), own_from);
+    int hi_warp = warp_has_rows ? ctx + token_of(last_row) : -1;
+    int lo_warp = max(first_visible_key(ctx + token_of(row0), p.window), own_from);
     // rows of the warp see every key of a chunk that lies in [all_lo, all_hi]: no mask needed
-    const int all_hi = warp_has_rows ? ctx + token_of(row0) : -1;
-    const int all_lo = first_visible_key(hi_warp, p.window);
+    int all_hi = warp_has_rows ? ctx + token_of(row0) : -1;
+    int all_lo = max(first_visible_key(hi_warp, p.window), own_from);
+    if (KEYS == SHARED_KEYS) {
+        // the rows' tokens are of many sequences: nothing follows from their order
+        const int first_token = token_of(tile_row0);
+        const KeyRange range = shared_keys_of_tokens(p.shared, q_start + first_token, token_of(tile_last) - first_token + 1, p.window, lane);
+        hi_tile = range.last;
+        lo_tile = range.first;
+        hi_warp = warp_has_rows ? __reduce_max_sync(0xffffffffu, max(r_pos[0], r_pos[1])) : -1;
+        lo_warp = __reduce_min_sync(0xffffffffu, min(r_lo[0], r_lo[1]));
+        all_hi = warp_has_rows ? __reduce_min_sync(0xffffffffu, min(r_pos[0], r_pos[1])) : -1;
+        all_lo = __reduce_max_sync(0xffffffffu, max(r_lo[0], r_lo[1]));
+    }
     const bool rows_full = row0 + 15 < n_rows;
     // keys [0, kept) are seen beside the window's: their chunks that lie wholly before the window's first one
     // are walked first. The walk counts v = 0 .. n_chunks - 1: chunk v for v < n_kept, then the window's chunks.
     const int kept = lo_tile > 0 ? min(p.keep_first, lo_tile) : 0;
     const int first_chunk = lo_tile / CHUNK, last_chunk = hi_tile / CHUNK;
     const int n_kept = min((kept + CHUNK - 1) / CHUNK, first_chunk);
-    const int n_chunks = n_kept + last_chunk - first_chunk + 1;
+    const int n_chunks = KEYS != ALL_KEYS && hi_tile < lo_tile ? 0 : n_kept + last_chunk - first_chunk + 1;
     const int per_split = (n_chunks + p.n_splits - 1) / p.n_splits;
     const int c_begin = split * per_split;
     const int c_end = min(n_chunks, c_begin + per_split);
@@ -350,7 +394,7 @@ attention_mma_kernel(const MmaAttnParams p) {
         issue_chunk_warp<HD>(p, my_stages, my_stages + CHUNK * HD, &my_bars[0], chunk_of(my_first) * CHUNK, lo_tile,
                              hi_tile, kept, bt, kbase, vbase, page_stride, lane, cached_for(0));
     // queries and the newest keys and values come from the kernels before this one
-    pdl_wait();
+    if (KEYS == ALL_KEYS || (KEYS == OWN_KEYS && !p.shared.beside)) pdl_wait();
     if (p.beside) pdl_trigger();                        // what was waited for is now there for the next kernel too
     // Q fragments: 16 bytes of each owned row per 32-wide block. A row beyond the tile reads the
     // tile's last row (r_tok, r_head point there): its scores are masked and it is never written, and
@@ -567,6 +611,11 @@ attention_mma_kernel(const MmaAttnParams p) {
                 }
         }
     };
+    // where this block's part of a token and head goes
+    auto part_of = [&](int tok, int head) {
+        const size_t pair = (size_t)(q_start + tok) * p.n_heads + head;
+        return KEYS == ALL_KEYS ? pair * p.n_splits + split : pair * p.shared.n_parts + p.part + split;
+    };
     if (NARROW) {
         // ---- each warp streams chunks c_begin + warp, + 8, ... through a stage of its own: with eight
         // warps a block has eight chunks in flight, and a warp fetches its next chunk when it is done with
@@ -631,7 +680,8 @@ attention_mma_kernel(const MmaAttnParams p) {
             for (int w = 0; w < NARROW_WARPS; ++w) l += red_ml[((size_t)w * 16 + tid) * 2 + 1] * weight_of[w][tid];
             sum_of[tid] = l;
         }
-        if (p.n_splits == 1) __syncthreads();      // the only reader of sum_of among other threads
+        const bool whole = KEYS == ALL_KEYS && p.n_splits == 1;
+        if (whole) __syncthreads();                // the only reader of sum_of among other threads
         const int rows_here = min(16, n_rows - tile_row0);
         const float ln2 = 0.6931471805599453f;
         for (int idx = tid; idx < rows_here * (HD / 4); idx += NARROW_THREADS) {
@@ -645,7 +695,7 @@ attention_mma_kernel(const MmaAttnParams p) {
             }
             const int row = tile_row0 + r;
             const int tok = token_of(row), head = kh * group + (row - tok * group);
-            if (p.n_splits == 1) {
+            if (whole) {
                 // the sink counts once in the denominator (maxima are in units of log2)
                 const float inv = 1.f / (sum_of[r] + (p.sink ? fast_exp2(p.sink[head] * 1.4426950408889634f - max_of[r]) : 0.f));
                 uint2 packed;
@@ -653,17 +703,18 @@ attention_mma_kernel(const MmaAttnParams p) {
                 packed.y = pack_bf16(acc.z * inv, acc.w * inv);
                 *reinterpret_cast<uint2*>(p.out + (size_t)(q_start + tok) * p.out_stride + (size_t)head * HD + d) = packed;
             } else {
-                const size_t base = ((size_t)(q_start + tok) * p.n_heads + head) * p.n_splits + split;
+                const size_t base = part_of(tok, head);
                 *reinterpret_cast<float4*>(p.part_o + base * HD + d) = acc;
             }
         }
-        if (p.n_splits > 1 && tid < rows_here) {
+        if (!whole && tid < rows_here) {
             const int row = tile_row0 + tid;
             const int tok = token_of(row), head = kh * group + (row - tok * group);
-            const size_t base = ((size_t)(q_start + tok) * p.n_heads + head) * p.n_splits + split;
+            const size_t base = part_of(tok, head);
             p.part_ml[base * 2] = max_of[tid] * ln2;     // the merge kernel works with natural logs
             p.part_ml[base * 2 + 1] = sum_of[tid];
         }
+        if (KEYS == OWN_KEYS) pdl_wait();                // whoever waits for this kernel waits for the shared keys' too
         return;
     }
 
@@ -685,7 +736,9 @@ attention_mma_kernel(const MmaAttnParams p) {
         // the chunks of a pair need not be neighbours: the last of the kept first tokens and the window's first
         const bool two = ci + 1 < c_end;
         const int c0 = chunk_of(ci) * CHUNK, c1 = two ? chunk_of(ci + 1) * CHUNK : c0;
-        if (!(warp_has_rows && c0 <= hi_warp && (c1 + CHUNK - 1 >= lo_warp || c0 < kept))) continue;
+        // (of rows that are of many sequences no two warps' keys need to meet: a pair of chunks that every warp left out would
+        // be overwritten while it is still on its way)
+        if (!(warp_has_rows && (KEYS == SHARED_KEYS || (c0 <= hi_warp && (c1 + CHUNK - 1 >= lo_warp || c0 < kept))))) continue;
         const int st0 = i % WIDE_STAGES, st1 = (i + 1) % WIDE_STAGES;
         const __nv_bfloat16* ks0 = stages + (size_t)st0 * STAGE_ELEMS;
         const __nv_bfloat16* ks1 = stages + (size_t)st1 * STAGE_ELEMS;
@@ -699,7 +752,7 @@ attention_mma_kernel(const MmaAttnParams p) {
     }
 
     // each warp writes its own rows; this thread holds columns 8 nb + 2t, + 1 of rows g, g + 8
-    if (p.n_splits == 1) {
+    if (KEYS == ALL_KEYS && p.n_splits == 1) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (!r_valid[i]) continue;
@@ -716,8 +769,7 @@ attention_mma_kernel(const MmaAttnParams p) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (!r_valid[i]) continue;
-            const size_t base = ((size_t)(q_start + r_tok[i]) * p.n_heads + kh * group + r_head[i]) *
-                                    p.n_splits + split;
+            const size_t base = part_of(r_tok[i], kh * group + r_head[i]);
             float* po = p.part_o + base * HD;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
@@ -730,9 +782,10 @@ attention_mma_kernel(const MmaAttnParams p) {
             }
         }
     }
+    if (KEYS == OWN_KEYS) pdl_wait();
 }
 
-template <int HD, bool NARROW, bool BIASED>
+template <int HD, bool NARROW, bool BIASED, Keys KEYS>
 int launch_mma_kernel(const MmaAttnParams& p, cudaStream_t stream) {
     const size_t stage_bytes = 2 * (size_t)CHUNK * HD * sizeof(__nv_bfloat16);
     size_t smem = stage_bytes * (NARROW ? NARROW_STAGES * NARROW_WARPS : WIDE_STAGES);
@@ -741,18 +794,27 @@ int launch_mma_kernel(const MmaAttnParams& p, cudaStream_t stream) {
         if (reduce > smem) smem = reduce;
     }
     if (smem + 1024 > 48 * 1024) {   // the kernel also has a little static shared memory
-        cudaError_t e = cudaFuncSetAttribute(attention_mma_kernel<HD, NARROW, BIASED>,
+        cudaError_t e = cudaFuncSetAttribute(attention_mma_kernel<HD, NARROW, BIASED, KEYS>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) MX_REFUSE("attention: cannot reserve %zu bytes of shared memory", smem);
     }
     dim3 grid(p.n_tiles, p.n_kv_heads, p.n_splits);
-    mx_launch_chained(attention_mma_kernel<HD, NARROW, BIASED>, grid, dim3(NARROW ? NARROW_THREADS : MMA_THREADS), smem, stream, p);
+    if (KEYS == OWN_KEYS && p.shared.beside) {
+        const cudaError_t e = mx_launch_beside(attention_mma_kernel<HD, NARROW, BIASED, KEYS>, grid,
+                                               dim3(NARROW ? NARROW_THREADS : MMA_THREADS), smem, stream, p);
+        if (e != cudaSuccess) {
+            mx_set_error("attention: launch failed: %s", cudaGetErrorString(e));
+            return (int)e;
+        }
+        return MX_OK;
+    }
+    mx_launch_chained(attention_mma_kernel<HD, NARROW, BIASED, KEYS>, grid, dim3(NARROW ? NARROW_THREADS : MMA_THREADS), smem, stream, p);
     return mx_launch_status();
 }
 
 template <int HD, bool NARROW>
 int launch_mma(const MmaAttnParams& p, cudaStream_t stream) {
-    return p.distance ? launch_mma_kernel<HD, NARROW, true>(p, stream) : launch_mma_kernel<HD, NARROW, false>(p, stream);
+    return p.distance ? launch_mma_kernel<HD, NARROW, true, ALL_KEYS>(p, stream) : launch_mma_kernel<HD, NARROW, false, ALL_KEYS>(p, stream);
 }
 
 }  // namespace
@@ -828,4 +890,31 @@ extern "C" int mx_paged_attention_mma(const void* q, int q_stride, const void* c
     if (rc != MX_OK || n_splits == 1) return rc;
     return mx_attention_merge_bf16_sink(p.part_o, p.part_ml, out, out_stride, n_tokens, n_heads, head_dim,
                                         n_splits, sink, stream);
+}
+
+// One half of attention_shared.cu: the keys that a group has in common (shared_keys; tiles of 64 rows of a group) or those of
+// each sequence alone (`narrow`: a tile is a whole sequence of at most 16 rows; else tiles of 64). `n_tiles`: the most that
+// there can be. Parts part .. part + n_splits - 1 are written.
+int mx_attention_mma_shared(const void* q, int q_stride, const void* cache, long long n_pages, int page_size,
+                            const int* block_tables, int bt_stride, const int* cu_q, const int* context_lens, int n_heads,
+                            int n_kv_heads, int head_dim, int window, float scale, float softcap, bool shared_keys, bool narrow,
+                            int n_tiles, int n_splits, int part, float* part_o, float* part_ml,
+                            const SharedPrefixParams& shared, int* status, cudaStream_t stream) {
+    MmaAttnParams p = {};
+    p.q = (const __nv_bfloat16*)q; p.cache = (const __nv_bfloat16*)cache; p.part_o = part_o; p.part_ml = part_ml;
+    p.block_tables = block_tables; p.cu_q = cu_q; p.context_lens = context_lens; p.status = status; p.n_pages = n_pages;
+    p.n_tiles = n_tiles; p.q_stride = q_stride; p.bt_stride = bt_stride; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads;
+    p.group = n_heads / n_kv_heads; p.page_size = page_size; p.page_shift = page_size == 8 ? 3 : (page_size == 16 ? 4 : 5);
+    p.window = window; p.n_splits = n_splits; p.scale_log2 = scale * 1.4426950408889634f;
+    p.cap_log2 = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
+    p.cap_in = softcap > 0.f ? scale / softcap : 0.f;
+    p.shared = shared;
+    p.part = part;
+    if (head_dim == 64)
+        return shared_keys ? launch_mma_kernel<64, false, false, SHARED_KEYS>(p, stream)
+               : narrow    ? launch_mma_kernel<64, true, false, OWN_KEYS>(p, stream)
+                           : launch_mma_kernel<64, false, false, OWN_KEYS>(p, stream);
+    return shared_keys ? launch_mma_kernel<128, false, false, SHARED_KEYS>(p, stream)
+           : narrow    ? launch_mma_kernel<128, true, false, OWN_KEYS>(p, stream)
+                       : launch_mma_kernel<128, false, false, OWN_KEYS>(p, stream);
 }

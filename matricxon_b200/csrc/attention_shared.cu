@@ -1,0 +1,470 @@
+// Paged attention for a step whose sequences lie in groups with their first keys in common (a system prompt, one document
+// and many questions): those keys are read once for all tokens of a group.
+//
+// Same mathematics and visibility rule as attention.cu (query at p sees key j iff j <= p and (window == 0 or j > p - window);
+// scores q.k * scale, optionally capped; float softmax, with a sink in its denominator where the caller has one). The softmax
+// of a (token, head) is cut into parts over disjoint keys, each with its maximum m_i, its sum l_i of exp(score - m_i) and its
+// weighted values o_i, in float:
+//   shared parts   the keys below lens[sequence], through the block table of the group's first sequence. The rows of an MMA
+//                  tile are (token, head) pairs of the whole group, whatever sequence a token is of;
+//   own parts      the keys from there on, through the sequence's own table;
+//   joined         m = max m_i, w_i = exp(m_i - m), out = sum w_i o_i / (sum w_i l_i + exp(sink - m)), rounded once.
+// Which kernels: bfloat16 heads of 128 on pages of 16 or 32 take tcgen05 for the shared keys (attention_tc.cu), other
+// bfloat16 heads of 64 and 128 mma.sync (attention_mma.cu), whose tiles of 16 or 64 rows also walk the own keys; everything
+// else (float, other head sizes) the kernel below, tiles of sixteen rows on the FP32 cores.
+// The two halves run at a time: the kernel of the shared keys waits for the queries and lets that of the own keys begin at
+// once, beside it; that one ends only when the first has, so the join waits for both.
+// Rows behind the last sequence's are read and written by nobody.
+#include <math.h>
+
+#include "common.cuh"
+#include "shared_prefix.cuh"
+
+namespace {
+
+constexpr int SH_THREADS = 128;
+constexpr int SH_WARPS = SH_THREADS / 32;
+constexpr int SH_KEYS = 32;                // keys a chunk, one a lane
+constexpr int SH_ROWS = 16;                // (token, head) rows a block
+constexpr int SH_ROWS_PER_WARP = SH_ROWS / SH_WARPS;
+
+struct SharedAttnParams {
+    const void *q, *cache;
+    float *part_o, *part_ml;
+    const int *block_tables, *cu_q;
+    int* status;
+    long long n_pages;
+    int q_stride, bt_stride, n_tokens, n_heads, n_kv_heads, group, head_dim, page_size, window, n_splits, part;
+    float scale, softcap;
+    SharedPrefixParams shared;
+};
+
+template <typename T> struct Vec16;        // 16 bytes of T
+template <> struct Vec16<float> { static constexpr int E = 4; };
+template <> struct Vec16<__nv_bfloat16> { static constexpr int E = 8; };
+
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4& raw, float* f);
+template <>
+__device__ __forceinline__ void unpack16<float>(const uint4& raw, float* f) {
+    f[0] = __uint_as_float(raw.x); f[1] = __uint_as_float(raw.y);
+    f[2] = __uint_as_float(raw.z); f[3] = __uint_as_float(raw.w);
+}
+template <>
+__device__ __forceinline__ void unpack16<__nv_bfloat16>(const uint4& raw, float* f) {
+    const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+
+// SHARED: a tile is sixteen (token, head) rows of a group, token-major. Otherwise up to sixteen heads of one token.
+template <typename T, int SLOTS, bool SHARED>
+__global__ void __launch_bounds__(SH_THREADS)
+shared_simt_kernel(const SharedAttnParams p) {
+    constexpr int E = Vec16<T>::E;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    __shared__ int row_token[SH_ROWS], row_head[SH_ROWS], row_lo[SH_ROWS], row_hi[SH_ROWS];
+    __shared__ float row_alpha[SH_ROWS], row_m[SH_ROWS], row_l[SH_ROWS];
+    const int hd = p.head_dim, cpr = hd / E;                  // 16-byte pieces a key
+    const int swz_mask = (cpr % 8 == 0) ? 7 : 0;
+    float* q_s = reinterpret_cast<float*>(smem_raw);          // [SH_ROWS][hd]
+    float* p_s = q_s + SH_ROWS * hd;                          // [SH_ROWS][SH_KEYS]
+    uint4* k_s = reinterpret_cast<uint4*>(p_s + SH_ROWS * SH_KEYS);   // [SH_KEYS][cpr], swizzled
+    uint4* v_s = k_s + SH_KEYS * cpr;                         // [SH_KEYS][cpr]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int kh = blockIdx.y, split = blockIdx.z;
+
+    pdl_wait();
+    pdl_trigger();
+    int seq, rows, first_token, first_row;
+    if (SHARED) {
+        const GroupTile found = find_group_tile(p.shared, p.cu_q, blockIdx.x, SH_ROWS, p.group, lane);
+        if (found.tokens <= 0) return;
+        seq = found.seq; first_token = found.q_start; first_row = found.first;
+        rows = min(SH_ROWS, found.tokens * p.group - first_row);
+    } else {
+        const int parts = (p.group + SH_ROWS - 1) / SH_ROWS;
+        first_token = blockIdx.x / parts;
+        first_row = (blockIdx.x - first_token * parts) * SH_ROWS;
+        rows = min(SH_ROWS, p.group - first_row);
+        if (first_token >= p.cu_q[p.shared.n_seqs]) return;
+        seq = p.shared.tok_seq[first_token];
+        if (seq < 0 || seq >= p.shared.n_seqs) return;
+    }
+    if (tid < rows) {
+        const int r = first_row + tid, t = r / p.group;
+        row_token[tid] = first_token + t;
+        row_head[tid] = kh * p.group + r - t * p.group;
+        if (SHARED) {
+            const KeyRange range = shared_keys_of_token(p.shared, first_token + t, p.window);
+            row_lo[tid] = range.first;
+            row_hi[tid] = range.last;
+        } else {
+            const int position = p.shared.positions[first_token];
+            row_lo[tid] = max(first_visible_key(position, p.window), p.shared.lens != nullptr ? p.shared.lens[seq] : 0);
+            row_hi[tid] = position;
+        }
+    }
+    __syncthreads();
+    int lo = 0x7fffffff, hi = -1;                             // the keys that any row sees
+    for (int r = 0; r < rows; ++r)
+        if (row_lo[r] <= row_hi[r]) { lo = min(lo, row_lo[r]); hi = max(hi, row_hi[r]); }
+    const int first_chunk = hi < lo ? 0 : lo / SH_KEYS, n_chunks = hi < lo ? 0 : hi / SH_KEYS + 1 - first_chunk;
+    const int per_split = (n_chunks + p.n_splits - 1) / p.n_splits;
+    const int c_begin = split * per_split, c_end = min(n_chunks, c_begin + per_split);
+
+    for (int i = tid; i < rows * hd; i += SH_THREADS) {
+        const int r = i / hd, d = i - r * hd;
+        q_s[i] = to_float(reinterpret_cast<const T*>(p.q)[(size_t)row_token[r] * p.q_stride + (size_t)row_head[r] * hd + d]);
+    }
+    float acc[SH_ROWS][SLOTS];
+#pragma unroll
+    for (int r = 0; r < SH_ROWS; ++r)
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) acc[r][s] = 0.f;
+    float m_run[SH_ROWS_PER_WARP], l_run[SH_ROWS_PER_WARP];
+#pragma unroll
+    for (int i = 0; i < SH_ROWS_PER_WARP; ++i) { m_run[i] = -INFINITY; l_run[i] = 0.f; }
+
+    const int* bt = p.block_tables + (size_t)seq * p.bt_stride;
+    const T* cache = reinterpret_cast<const T*>(p.cache);
+    const size_t head_stride = (size_t)p.page_size * hd;
+    for (int c = c_begin; c < c_end; ++c) {
+        const int c0 = (first_chunk + c) * SH_KEYS;
+        // ---- keys (zeros for those that no row sees)
+        for (int item = tid; item < SH_KEYS * cpr; item += SH_THREADS) {
+            const int j = item / cpr, piece = item - j * cpr, key = c0 + j;
+            uint4 raw = make_uint4(0, 0, 0, 0);
+            if (key >= lo && key <= hi) {
+                const int lp = key / p.page_size;
+                const long long page = lp < p.bt_stride ? bt[lp] : -1;
+                if (page < 0 || page >= p.n_pages) {
+                    if (piece == 0) atomicOr(p.status, MX_STATUS_BAD_PAGE);
+                } else {
+                    raw = *reinterpret_cast<const uint4*>(cache + ((size_t)page * 2 * p.n_kv_heads + kh) * head_stride +
+                                                          (size_t)(key - lp * p.page_size) * hd + (size_t)piece * E);
+                }
+            }
+            k_s[j * cpr + (piece ^ (j & swz_mask))] = raw;
+        }
+        // ---- values: memory has [dim][slot], shared memory wants [key][dim]; runs of E keys lie inside a page
+        {
+            constexpr int RUNS = SH_KEYS / E;
+            T* v_t = reinterpret_cast<T*>(v_s);
+            for (int item = tid; item < hd * RUNS; item += SH_THREADS) {
+                const int d = item / RUNS, run = item - d * RUNS, key0 = c0 + run * E;
+                uint4 raw = make_uint4(0, 0, 0, 0);
+                if (key0 <= hi && key0 + E - 1 >= lo) {
+                    const int lp = key0 / p.page_size;
+                    const long long page = lp < p.bt_stride ? bt[lp] : -1;
+                    if (page >= 0 && page < p.n_pages)
+                        raw = *reinterpret_cast<const uint4*>(cache + ((size_t)page * 2 * p.n_kv_heads + p.n_kv_heads + kh) * head_stride +
+                                                              (size_t)d * p.page_size + (key0 - lp * p.page_size));
+                }
+                const T* elems = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    v_t[(size_t)(run * E + e) * hd + d] = key0 + e >= lo && key0 + e <= hi ? elems[e] : from_float<T>(0.f);
+            }
+        }
+        __syncthreads();
+        // ---- scores: a lane a key, this warp's rows are warp, warp + 4, ...
+        float s[SH_ROWS_PER_WARP];
+#pragma unroll
+        for (int i = 0; i < SH_ROWS_PER_WARP; ++i) s[i] = 0.f;
+        for (int piece = 0; piece < cpr; ++piece) {
+            float kf[E];
+            unpack16<T>(k_s[lane * cpr + (piece ^ (lane & swz_mask))], kf);
+#pragma unroll
+            for (int i = 0; i < SH_ROWS_PER_WARP; ++i) {
+                const int r = warp + i * SH_WARPS;
+                if (r < rows) {
+                    const float4* qv = reinterpret_cast<const float4*>(q_s + r * hd + piece * E);
+#pragma unroll
+                    for (int e4 = 0; e4 < E / 4; ++e4) {
+                        const float4 qq = qv[e4];
+                        s[i] = fmaf(qq.x, kf[4 * e4 + 0], s[i]);
+                        s[i] = fmaf(qq.y, kf[4 * e4 + 1], s[i]);
+                        s[i] = fmaf(qq.z, kf[4 * e4 + 2], s[i]);
+                        s[i] = fmaf(qq.w, kf[4 * e4 + 3], s[i]);
+                    }
+                }
+            }
+        }
+        const int key = c0 + lane;
+#pragma unroll
+        for (int i = 0; i < SH_ROWS_PER_WARP; ++i) {
+            const int r = warp + i * SH_WARPS;
+            if (r < rows) {
+                const bool valid = key >= row_lo[r] && key <= row_hi[r];
+                float sv = s[i] * p.scale;
+                if (p.softcap > 0.f) sv = p.softcap * tanhf(sv / p.softcap);
+                sv = valid ? sv : -INFINITY;
+                const float m_new = fmaxf(m_run[i], warp_max(sv));
+                const float pj = valid ? expf(sv - m_new) : 0.f;
+                const float alpha = m_run[i] == -INFINITY ? 0.f : expf(m_run[i] - m_new);
+                l_run[i] = l_run[i] * alpha + warp_sum(pj);
+                m_run[i] = m_new;
+                p_s[r * SH_KEYS + lane] = pj;
+                if (lane == 0) row_alpha[r] = alpha;
+            }
+        }
+        __syncthreads();
+        // ---- weighted values: a thread a dimension (or two), all rows
+#pragma unroll
+        for (int slot = 0; slot < SLOTS; ++slot) {
+            const int d = tid + slot * SH_THREADS;
+            if (d < hd) {
+#pragma unroll
+                for (int r = 0; r < SH_ROWS; ++r)
+                    if (r < rows) acc[r][slot] *= row_alpha[r];
+                const T* vcol = reinterpret_cast<const T*>(v_s) + d;
+                for (int j = 0; j < SH_KEYS; j += 4) {
+                    const float v0 = to_float(vcol[(size_t)(j + 0) * hd]), v1 = to_float(vcol[(size_t)(j + 1) * hd]);
+                    const float v2 = to_float(vcol[(size_t)(j + 2) * hd]), v3 = to_float(vcol[(size_t)(j + 3) * hd]);
+#pragma unroll
+                    for (int r = 0; r < SH_ROWS; ++r)
+                        if (r < rows) {
+                            const float4 pp = *reinterpret_cast<const float4*>(p_s + r * SH_KEYS + j);
+                            acc[r][slot] = fmaf(pp.w, v3, fmaf(pp.z, v2, fmaf(pp.y, v1, fmaf(pp.x, v0, acc[r][slot]))));
+                        }
+                }
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < SH_ROWS_PER_WARP; ++i) {
+        const int r = warp + i * SH_WARPS;
+        if (r < rows && lane == 0) { row_m[r] = m_run[i]; row_l[r] = l_run[i]; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < SH_ROWS; ++r)
+        if (r < rows) {
+            const size_t base = ((size_t)row_token[r] * p.n_heads + row_head[r]) * p.shared.n_parts + p.part + split;
+#pragma unroll
+            for (int slot = 0; slot < SLOTS; ++slot) {
+                const int d = tid + slot * SH_THREADS;
+                if (d < hd) p.part_o[base * hd + d] = acc[r][slot];
+            }
+            if (tid == 0) { p.part_ml[base * 2] = row_m[r]; p.part_ml[base * 2 + 1] = row_l[r]; }
+        }
+}
+
+// The join: a warp a (token, head), four dimensions a lane. A token of no sequence is left alone.
+constexpr int JOIN_WARPS = 4;
+template <typename T>
+__global__ void __launch_bounds__(JOIN_WARPS * 32)
+shared_join_kernel(const float* part_o, const float* part_ml, T* out, int out_stride, const int* cu_q, const float* sink,
+                   int n_heads, int head_dim, long long n_pairs, const SharedPrefixParams shared) {
+    pdl_trigger();
+    const long long pair = (long long)blockIdx.x * JOIN_WARPS + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    pdl_wait();
+    if (pair >= n_pairs) return;
+    part_o = after_wait(part_o);
+    part_ml = after_wait(part_ml);
+    const int token = (int)(pair / n_heads), head = (int)(pair - (long long)token * n_heads);
+    if (token >= cu_q[shared.n_seqs]) return;
+    const size_t base = (size_t)pair * shared.n_parts;
+    float m = -INFINITY;
+    for (int s = lane; s < shared.n_parts; s += 32) m = fmaxf(m, part_ml[(base + s) * 2]);
+    m = warp_max(m);
+    float total = 0.f;
+    float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    for (int s0 = 0; s0 < shared.n_parts; s0 += 32) {
+        const int s = s0 + lane;
+        const float2 ml = s < shared.n_parts ? *reinterpret_cast<const float2*>(part_ml + (base + s) * 2) : make_float2(-INFINITY, 0.f);
+        const float weight = ml.x == -INFINITY ? 0.f : expf(ml.x - m);
+        total += warp_sum(ml.y * weight);
+        for (int j = 0; j < min(32, shared.n_parts - s0); ++j) {
+            const float w = __shfl_sync(0xffffffffu, weight, j);
+            if (w == 0.f) continue;                // a part without keys has values nobody wrote
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int d = 4 * lane + 128 * i;
+                if (d < head_dim) {
+                    const float4 v = *reinterpret_cast<const float4*>(part_o + (base + s0 + j) * head_dim + d);
+                    o[i].x = fmaf(v.x, w, o[i].x); o[i].y = fmaf(v.y, w, o[i].y);
+                    o[i].z = fmaf(v.z, w, o[i].z); o[i].w = fmaf(v.w, w, o[i].w);
+                }
+            }
+        }
+    }
+    if (sink) total += expf(sink[head] - m);
+    const float inv = 1.f / total;
+    T* dst = out + (size_t)token * out_stride + (size_t)head * head_dim;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int d = 4 * lane + 128 * i;
+        if (d < head_dim) {
+            dst[d] = from_float<T>(o[i].x * inv); dst[d + 1] = from_float<T>(o[i].y * inv);
+            dst[d + 2] = from_float<T>(o[i].z * inv); dst[d + 3] = from_float<T>(o[i].w * inv);
+        }
+    }
+}
+
+template <typename T, int SLOTS, bool SHARED>
+int launch_simt(const SharedAttnParams& p, unsigned n_tiles, cudaStream_t stream) {
+    const size_t smem = (size_t)SH_ROWS * p.head_dim * 4 + SH_ROWS * SH_KEYS * 4 + 2 * (size_t)SH_KEYS * p.head_dim * sizeof(T);
+    if (smem > 47 * 1024 && cudaFuncSetAttribute(shared_simt_kernel<T, SLOTS, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)smem) != cudaSuccess)
+        MX_REFUSE("attention over shared keys: cannot reserve %zu bytes of shared memory", smem);
+    const cudaError_t e = mx_launch_chained(shared_simt_kernel<T, SLOTS, SHARED>, dim3(n_tiles, p.n_kv_heads, p.n_splits),
+                                            dim3(SH_THREADS), smem, stream, p);
+    if (e != cudaSuccess) {
+        mx_set_error("attention over shared keys: launch failed: %s", cudaGetErrorString(e));
+        return (int)e;
+    }
+    return MX_OK;
+}
+
+template <typename T>
+int launch_join(const SharedAttnParams& p, T* out, int out_stride, const float* sink, cudaStream_t stream) {
+    const long long pairs = (long long)p.n_tokens * p.n_heads;
+    const cudaError_t e = mx_launch_beside(shared_join_kernel<T>, dim3((unsigned)((pairs + JOIN_WARPS - 1) / JOIN_WARPS)),
+                                           dim3(JOIN_WARPS * 32), 0, stream, (const float*)p.part_o, (const float*)p.part_ml, out, out_stride,
+                                           p.cu_q, sink, p.n_heads, p.head_dim, pairs, p.shared);
+    if (e != cudaSuccess) {
+        mx_set_error("attention over shared keys: launch failed: %s", cudaGetErrorString(e));
+        return (int)e;
+    }
+    return MX_OK;
+}
+
+// How the launch is cut up. tcgen05 tiles, mma tiles or the FP32 cores (`path` 2, 1, 0), the most tiles there can be of either
+// kind, and into how many parts the shared and the own keys of a tile are dealt out.
+struct SharedPlan {
+    int path, shared_tiles, own_tiles, shared_parts, own_parts;
+    bool narrow;
+};
+
+SharedPlan make_plan(int dtype, int head_dim, int page_size, bool aligned, int n_tokens, int n_heads, int n_kv_heads, int n_seqs,
+                     int n_groups, int max_q_len, int max_shared_len, int max_own_len, int n_sm) {
+    SharedPlan plan;
+    const int group = n_heads / n_kv_heads;
+    const bool mma = dtype == MX_DTYPE_BF16 && aligned && (head_dim == 64 || head_dim == 128) &&
+                     (page_size == 8 || page_size == 16 || page_size == 32);
+    const bool tc = mma && head_dim == 128 && page_size != 8 && group <= 128;
+    plan.path = tc ? 2 : (mma ? 1 : 0);
+    const long long rows = (long long)n_tokens * group;
+    plan.narrow = mma && (long long)max_q_len * group <= 16;
+    const int shared_rows = tc ? 128 / group * group : (mma ? 64 : SH_ROWS);
+    plan.shared_tiles = (int)min(rows / shared_rows + n_groups, rows);
+    plan.own_tiles = mma ? (plan.narrow ? n_seqs : (int)min(rows / 64 + n_seqs, rows)) : n_tokens * ((group + SH_ROWS - 1) / SH_ROWS);
+    const int shared_keys = tc ? 128 : 32;
+    const int shared_chunks = (max(max_shared_len, 1) + shared_keys - 1) / shared_keys, own_chunks = max(max_own_len, 1) / 32 + 1;
+    const int shared_blocks = plan.shared_tiles * n_kv_heads, own_blocks = plan.own_tiles * n_kv_heads;
+    plan.shared_parts = max_shared_len <= 0 ? 0 : max(1, min(min((tc ? n_sm : 4 * n_sm) / max(shared_blocks, 1), shared_chunks / (tc ? 2 : 4)), 32));
+    plan.own_parts = max(1, min(min((plan.narrow ? n_sm : 4 * n_sm) / max(own_blocks, 1), own_chunks / 8), 32));
+    return plan;
+}
+
+bool rows_aligned(const void* q, int q_stride, const void* cache) {
+    return q_stride % 8 == 0 && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache)) & 15) == 0;
+}
+
+}  // namespace
+
+int mx_attention_tc_shared(const void* q, int q_stride, const void* cache, long long n_pages, int page_size,
+                           const int* block_tables, int bt_stride, const int* cu_q, int n_tokens, int n_heads, int n_kv_heads,
+                           int window, float scale, float softcap, int n_tiles, int n_splits, float* part_o, float* part_ml,
+                           const SharedPrefixParams& shared, int* status, cudaStream_t stream);
+int mx_attention_mma_shared(const void* q, int q_stride, const void* cache, long long n_pages, int page_size,
+                            const int* block_tables, int bt_stride, const int* cu_q, const int* context_lens, int n_heads,
+                            int n_kv_heads, int head_dim, int window, float scale, float softcap, bool shared_keys, bool narrow,
+                            int n_tiles, int n_splits, int part, float* part_o, float* part_ml,
+                            const SharedPrefixParams& shared, int* status, cudaStream_t stream);
+
+// Bytes of scratch of mx_paged_attention_shared with the same arguments: the parts' values, maxima and sums. `aligned`: the
+// query rows and the pages start on 16 bytes.
+extern "C" long long mx_attention_shared_scratch(int dtype, int aligned, int page_size, int n_seqs, int n_groups, int n_tokens,
+                                                 int n_heads, int n_kv_heads, int head_dim, int max_q_len, int max_shared_len,
+                                                 int max_own_len, int n_sm) {
+    if (n_tokens <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || head_dim <= 0 || n_sm <= 0) return 0;
+    const SharedPlan plan = make_plan(dtype, head_dim, page_size, aligned != 0, n_tokens, n_heads, n_kv_heads, n_seqs, n_groups,
+                                      max_q_len, max_shared_len, max_own_len, n_sm);
+    return (long long)n_tokens * n_heads * (plan.shared_parts + plan.own_parts) * (head_dim + 2) * (long long)sizeof(float);
+}
+
+// max_q_len: no sequence brings more tokens. max_shared_len and max_own_len size the parts alone: smaller numbers than the true
+// ones cost time, not results (with max_shared_len 0 every key is read through its sequence's own table).
+extern "C" int mx_paged_attention_shared(const void* q, int dtype, int q_stride, const void* cache, long long n_pages,
+                                         int page_size, const int* block_tables, int bt_stride, const int* cu_q,
+                                         const int* context_lens, const int* tok_seq, const int* positions, const int* first,
+                                         const int* lens, int n_seqs, int n_groups, int n_tokens, int n_heads, int n_kv_heads,
+                                         int head_dim, int window, float scale, float softcap, const float* sink, void* out,
+                                         int out_stride, int max_q_len, int max_shared_len, int max_own_len, int n_sm,
+                                         float* scratch, int* status, cudaStream_t stream) {
+    if (n_tokens <= 0 || n_seqs <= 0) return MX_OK;
+    if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0)
+        MX_REFUSE("attention: %d heads are not a multiple of %d kv heads", n_heads, n_kv_heads);
+    if (head_dim % 16 != 0 || head_dim < 16 || head_dim > 256)
+        MX_REFUSE("attention: head_dim %d is not a multiple of 16 in [16, 256]", head_dim);
+    if (page_size <= 0 || page_size % 8 != 0) MX_REFUSE("attention: page size %d is not a positive multiple of 8", page_size);
+    if (n_kv_heads > 65535) MX_REFUSE("attention: %d kv heads exceed the grid", n_kv_heads);
+    if (max_q_len <= 0 || max_shared_len < 0 || max_own_len < 0 || n_sm <= 0)
+        MX_REFUSE("attention over shared keys: bounds of %d tokens, %d and %d keys", max_q_len, max_shared_len, max_own_len);
+    if ((long long)n_tokens * n_heads > 0x7fffffffLL) MX_REFUSE("attention over shared keys: %d tokens of %d heads", n_tokens, n_heads);
+    if (n_pages * 2 * n_kv_heads > 0x7fffffffLL) MX_REFUSE("attention over shared keys: %lld pages are too many", n_pages);
+    if (reinterpret_cast<uintptr_t>(cache) % 16 != 0) MX_REFUSE("attention over shared keys needs 16-byte aligned pages");
+    if (scratch == nullptr || status == nullptr) MX_REFUSE("attention over shared keys needs scratch memory and a status word");
+    const SharedPlan plan = make_plan(dtype, head_dim, page_size, rows_aligned(q, q_stride, cache), n_tokens, n_heads, n_kv_heads,
+                                      n_seqs, n_groups, max_q_len, max_shared_len, max_own_len, n_sm);
+    SharedAttnParams p;
+    p.q = q; p.cache = cache; p.block_tables = block_tables; p.cu_q = cu_q; p.status = status; p.n_pages = n_pages;
+    p.q_stride = q_stride; p.bt_stride = bt_stride; p.n_tokens = n_tokens; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads;
+    p.group = n_heads / n_kv_heads; p.head_dim = head_dim; p.page_size = page_size; p.window = window; p.scale = scale;
+    p.softcap = softcap;
+    p.shared.first = first; p.shared.lens = lens; p.shared.tok_seq = tok_seq; p.shared.positions = positions;
+    p.shared.n_groups = n_groups; p.shared.n_seqs = n_seqs; p.shared.n_shared_parts = plan.shared_parts;
+    p.shared.n_parts = plan.shared_parts + plan.own_parts;
+    p.shared.beside = 0;
+    if (plan.shared_parts == 0) p.shared.lens = nullptr;
+    p.part_o = scratch;
+    p.part_ml = scratch + (size_t)n_tokens * n_heads * p.shared.n_parts * head_dim;
+    int rc = MX_OK;
+    if (plan.shared_parts > 0) {
+        if (plan.path == 2) {
+            rc = mx_attention_tc_shared(q, q_stride, cache, n_pages, page_size, block_tables, bt_stride, cu_q, n_tokens, n_heads,
+                                        n_kv_heads, window, scale, softcap, plan.shared_tiles, plan.shared_parts, p.part_o, p.part_ml,
+                                        p.shared, status, stream);
+        } else if (plan.path == 1) {
+            rc = mx_attention_mma_shared(q, q_stride, cache, n_pages, page_size, block_tables, bt_stride, cu_q, context_lens,
+                                         n_heads, n_kv_heads, head_dim, window, scale, softcap, true, false, plan.shared_tiles,
+                                         plan.shared_parts, 0, p.part_o, p.part_ml, p.shared, status, stream);
+        } else {
+            p.n_splits = plan.shared_parts;
+            p.part = 0;
+            if (dtype == MX_DTYPE_F32)
+                rc = head_dim > SH_THREADS ? launch_simt<float, 2, true>(p, plan.shared_tiles, stream)
+                                           : launch_simt<float, 1, true>(p, plan.shared_tiles, stream);
+            else
+                rc = head_dim > SH_THREADS ? launch_simt<__nv_bfloat16, 2, true>(p, plan.shared_tiles, stream)
+                                           : launch_simt<__nv_bfloat16, 1, true>(p, plan.shared_tiles, stream);
+        }
+        if (rc != MX_OK) return rc;
+        p.shared.beside = plan.path > 0;
+    }
+    if (plan.path > 0) {
+        rc = mx_attention_mma_shared(q, q_stride, cache, n_pages, page_size, block_tables, bt_stride, cu_q, context_lens, n_heads,
+                                     n_kv_heads, head_dim, window, scale, softcap, false, plan.narrow, plan.own_tiles, plan.own_parts,
+                                     plan.shared_parts, p.part_o, p.part_ml, p.shared, status, stream);
+    } else {
+        p.n_splits = plan.own_parts;
+        p.part = plan.shared_parts;
+        if (dtype == MX_DTYPE_F32)
+            rc = head_dim > SH_THREADS ? launch_simt<float, 2, false>(p, plan.own_tiles, stream)
+                                       : launch_simt<float, 1, false>(p, plan.own_tiles, stream);
+        else
+            rc = head_dim > SH_THREADS ? launch_simt<__nv_bfloat16, 2, false>(p, plan.own_tiles, stream)
+                                       : launch_simt<__nv_bfloat16, 1, false>(p, plan.own_tiles, stream);
+    }
+    if (rc != MX_OK) return rc;
+    if (dtype == MX_DTYPE_F32) return launch_join<float>(p, (float*)out, out_stride, sink, stream);
+    return launch_join<__nv_bfloat16>(p, (__nv_bfloat16*)out, out_stride, sink, stream);
+}

@@ -44,6 +44,7 @@
 #include <math.h>
 
 #include "common.cuh"
+#include "shared_prefix.cuh"
 
 namespace {
 
@@ -91,6 +92,7 @@ struct AtParams {
     float cap_log2, cap_in;
     const float* sink;           // [heads] or null: exp(sink[h]) joins the softmax's denominator, with no value
     const float* distance;       // [2][heads] (r1, then r2) or null: scores lose r1 ln(1 + r2 (p - j))
+    SharedPrefixParams shared;   // SHARED only
 };
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -236,7 +238,10 @@ __device__ __forceinline__ unsigned at_pack(float lo, float hi) {
     return *reinterpret_cast<unsigned*>(&v);
 }
 
-template <bool BIASED>
+// SHARED: the tiles are of a group's tokens, which have their first keys in common, and the keys are those alone
+// (attention_shared.cu): a tile's tokens may come from many sequences, the pages are those of the group's first one, each row
+// has limits of its own, and what comes out are always parts.
+template <bool BIASED, bool SHARED>
 __global__ void __launch_bounds__(AT_THREADS, 1)
 attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                     const __grid_constant__ CUtensorMap v_map, const AtParams p) {
@@ -260,17 +265,33 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     asm volatile("fence.proxy.async.global;\n" ::: "memory");
     const int tile = (int)(blockIdx.x / (unsigned)p.n_kv_heads);
     const int kh = (int)(blockIdx.x % (unsigned)p.n_kv_heads);
-    const int seq = p.tiles[2 * tile], tok0 = p.tiles[2 * tile + 1];
-    const int q_start = p.cu_q[seq];
-    const int q_len = p.cu_q[seq + 1] - q_start;
-    const int ctx = p.context_lens[seq];
+    int seq, tok0, q_start, q_len, ctx = 0;
+    if (SHARED) {
+        // the queries come from the kernel before; once that has ended, the launch after this one may begin beside it
+        pdl_wait();
+        pdl_trigger();
+        asm volatile("fence.proxy.async.global;\n" ::: "memory");
+        const GroupTile found = find_group_tile(p.shared, p.cu_q, tile, p.tokens_per_tile, 1, lane);
+        if (found.tokens <= 0) return;                              // more blocks than tiles
+        seq = found.seq; tok0 = found.first; q_start = found.q_start; q_len = found.tokens;
+    } else {
+        seq = p.tiles[2 * tile]; tok0 = p.tiles[2 * tile + 1];
+        q_start = p.cu_q[seq];
+        q_len = p.cu_q[seq + 1] - q_start;
+        ctx = p.context_lens[seq];
+    }
     const int n_tok = min(p.tokens_per_tile, q_len - tok0);
     if (n_tok <= 0) {                                               // nothing was allocated yet
         pdl_wait();
         return;
     }
-    const int hi_tile = ctx + tok0 + n_tok - 1;
-    const int lo_tile = first_visible_key(ctx + tok0, p.window);
+    int hi_tile = ctx + tok0 + n_tok - 1;
+    int lo_tile = first_visible_key(ctx + tok0, p.window);
+    if (SHARED) {
+        const KeyRange range = shared_keys_of_tokens(p.shared, q_start + tok0, n_tok, p.window, lane);
+        hi_tile = range.last;
+        lo_tile = range.first;
+    }
     // the tile's chunks of 128 keys, and this block's share of them when the keys are split (few tiles, a
     // long context: the shares are merged by mx_attention_merge_bf16); a share may be empty
     // With kept first tokens the tile walks two runs of chunks, the kept tokens' and the window's, as one list:
@@ -278,7 +299,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     // runs, 0 when they touch; without kept tokens kept_chunks is 0 and skipped the window's first chunk).
     const int kept_chunks = (p.window > 0 && p.keep > 0) ? (p.keep + AT_KEYS - 1) / AT_KEYS : 0;
     const int skipped = max(0, lo_tile / AT_KEYS - kept_chunks);
-    const int all_chunks = hi_tile / AT_KEYS + 1 - skipped;
+    const int all_chunks = SHARED && hi_tile < lo_tile ? 0 : hi_tile / AT_KEYS + 1 - skipped;
     const int per_split = (all_chunks + p.n_splits - 1) / p.n_splits;
     const int i_begin = (int)blockIdx.z * per_split;
     auto chunk_of = [&](int j) { const int i = i_begin + j; return i < kept_chunks ? i : i + skipped; };
@@ -287,7 +308,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         const int t_in = tid / p.group, h_in = tid - t_in * p.group;
         if (tid < p.tokens_per_tile * p.group && t_in < n_tok) {
             const size_t base = ((size_t)(q_start + tok0 + t_in) * p.n_heads + (size_t)(kh * p.group + h_in)) *
-                                    p.n_splits + blockIdx.z;
+                                    (SHARED ? p.shared.n_parts : p.n_splits) + blockIdx.z;
             p.part_ml[base * 2] = -INFINITY;
             p.part_ml[base * 2 + 1] = 0.f;
         }
@@ -461,8 +482,13 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         const int part = warp >> 2, row = tid & (AT_ROWS - 1);
         const int t_in = row / p.group, h_in = row - t_in * p.group;
         const bool valid = row < p.tokens_per_tile * p.group && t_in < n_tok;
-        const int pos = valid ? ctx + tok0 + t_in : -1;                 // -1: every key is masked
-        const int lo = first_visible_key(pos, p.window);
+        int pos = valid ? ctx + tok0 + t_in : -1;                       // -1: every key is masked
+        int lo = first_visible_key(pos, p.window);
+        if (SHARED && valid) {
+            const KeyRange range = shared_keys_of_token(p.shared, q_start + tok0 + t_in, p.window);
+            pos = range.last;
+            lo = range.first;
+        }
         const unsigned lane_base = (unsigned)(32 * (warp & 3)) << 16;
         const unsigned o_addr = tmem_o + 128 * part + lane_base;
         // distance bias of the row's head; a row that belongs to no token takes none (its scores stay numbers)
@@ -641,10 +667,10 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
 #pragma unroll
             for (int c = 0; c < 32; ++c) o[c] = fmaf(o[c], w0, other[c] * w1);
         };
-        if (alive && p.n_splits > 1) {
+        if (alive && (SHARED || p.n_splits > 1)) {
             // a share of the keys: the unnormalised sums, the reference maximum and the sum of weights
             const size_t base = ((size_t)(q_start + tok0 + t_in) * p.n_heads + (size_t)(kh * p.group + h_in)) *
-                                    p.n_splits + blockIdx.z;
+                                    (SHARED ? p.shared.n_parts : p.n_splits) + blockIdx.z;
             const bool any = l_run > 0.f;
             if (valid && part == 0) {
                 p.part_ml[base * 2] = any ? m_ref * 0.6931471805599453f : -INFINITY;
@@ -719,6 +745,47 @@ int at_make_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* 
     return MX_OK;
 }
 
+// The tensor maps of the queries (boxes of a tile's tokens), of the pages' keys and of their values.
+int at_make_maps(CUtensorMap* q_map, CUtensorMap* k_map, CUtensorMap* v_map, const void* q, int q_stride, const void* cache,
+                 long long n_pages, int page_size, int n_tokens, int n_kv_heads, int group) {
+    const int tokens_per_tile = AT_ROWS / group;
+    {
+        const cuuint64_t dims[4] = {(cuuint64_t)AT_HD, (cuuint64_t)group, (cuuint64_t)n_kv_heads, (cuuint64_t)n_tokens};
+        const cuuint64_t strides[3] = {(cuuint64_t)AT_HD * 2, (cuuint64_t)group * AT_HD * 2, (cuuint64_t)q_stride * 2};
+        const cuuint32_t box[4] = {64, (cuuint32_t)group, 1, (cuuint32_t)tokens_per_tile};
+        const int rc = at_make_map(q_map, q, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc != MX_OK) return rc;
+    }
+    const cuuint64_t blocks = (cuuint64_t)n_pages * 2 * n_kv_heads;
+    {
+        const cuuint64_t dims[3] = {(cuuint64_t)AT_HD, (cuuint64_t)page_size, blocks};
+        const cuuint64_t strides[2] = {(cuuint64_t)AT_HD * 2, (cuuint64_t)page_size * AT_HD * 2};
+        const cuuint32_t box[3] = {64, (cuuint32_t)page_size, 1};
+        const int rc = at_make_map(k_map, cache, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc != MX_OK) return rc;
+    }
+    {
+        const cuuint64_t dims[3] = {(cuuint64_t)page_size, (cuuint64_t)AT_HD, blocks};
+        const cuuint64_t strides[2] = {(cuuint64_t)page_size * 2, (cuuint64_t)page_size * AT_HD * 2};
+        const cuuint32_t box[3] = {(cuuint32_t)page_size, (cuuint32_t)AT_HD, 1};
+        const int rc = at_make_map(v_map, cache, 3, dims, strides, box,
+                                   page_size == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B);
+        if (rc != MX_OK) return rc;
+    }
+    return MX_OK;
+}
+
+template <bool BIASED, bool SHARED>
+int at_reserve(size_t smem) {
+    static bool attribute_set = false;
+    if (!attribute_set) {
+        if (cudaFuncSetAttribute(attention_tc_kernel<BIASED, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+            MX_REFUSE("tcgen05 attention: cannot reserve %zu bytes of shared memory", smem);
+        attribute_set = true;
+    }
+    return MX_OK;
+}
+
 }  // namespace
 
 
@@ -760,29 +827,8 @@ extern "C" int mx_paged_attention_tc_split(const void* q, int q_stride, const vo
     const int tokens_per_tile = AT_ROWS / group;
 
     CUtensorMap q_map, k_map, v_map;
-    {
-        const cuuint64_t dims[4] = {(cuuint64_t)AT_HD, (cuuint64_t)group, (cuuint64_t)n_kv_heads, (cuuint64_t)n_tokens};
-        const cuuint64_t strides[3] = {(cuuint64_t)AT_HD * 2, (cuuint64_t)group * AT_HD * 2, (cuuint64_t)q_stride * 2};
-        const cuuint32_t box[4] = {64, (cuuint32_t)group, 1, (cuuint32_t)tokens_per_tile};
-        const int rc = at_make_map(&q_map, q, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-        if (rc != MX_OK) return rc;
-    }
-    const cuuint64_t blocks = (cuuint64_t)n_pages * 2 * n_kv_heads;
-    {
-        const cuuint64_t dims[3] = {(cuuint64_t)AT_HD, (cuuint64_t)page_size, blocks};
-        const cuuint64_t strides[2] = {(cuuint64_t)AT_HD * 2, (cuuint64_t)page_size * AT_HD * 2};
-        const cuuint32_t box[3] = {64, (cuuint32_t)page_size, 1};
-        const int rc = at_make_map(&k_map, cache, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-        if (rc != MX_OK) return rc;
-    }
-    {
-        const cuuint64_t dims[3] = {(cuuint64_t)page_size, (cuuint64_t)AT_HD, blocks};
-        const cuuint64_t strides[2] = {(cuuint64_t)page_size * 2, (cuuint64_t)page_size * AT_HD * 2};
-        const cuuint32_t box[3] = {(cuuint32_t)page_size, (cuuint32_t)AT_HD, 1};
-        const int rc = at_make_map(&v_map, cache, 3, dims, strides, box,
-                                   page_size == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B);
-        if (rc != MX_OK) return rc;
-    }
+    const int mapped = at_make_maps(&q_map, &k_map, &v_map, q, q_stride, cache, n_pages, page_size, n_tokens, n_kv_heads, group);
+    if (mapped != MX_OK) return mapped;
     AtParams p;
     p.block_tables = block_tables; p.cu_q = cu_q; p.context_lens = context_lens; p.tiles = tiles;
     p.out = (__nv_bfloat16*)out; p.status = status; p.n_pages = n_pages; p.out_stride = out_stride;
@@ -798,14 +844,8 @@ extern "C" int mx_paged_attention_tc_split(const void* q, int q_stride, const vo
     p.part_o = scratch;
     p.part_ml = scratch ? scratch + (size_t)n_tokens * n_heads * n_splits * AT_HD : nullptr;
     const size_t smem = (size_t)(2 + 2 * AT_STAGES * 2) * AT_TILE + 1024;
-    static bool attribute_set = false;
-    if (!attribute_set) {
-        cudaError_t e = cudaFuncSetAttribute(attention_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(attention_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) MX_REFUSE("tcgen05 attention: cannot reserve %zu bytes of shared memory", smem);
-        attribute_set = true;
-    }
+    const int reserved = distance ? at_reserve<true, false>(smem) : at_reserve<false, false>(smem);
+    if (reserved != MX_OK) return reserved;
     if ((long long)n_tiles * n_kv_heads > 0x7fffffffLL) MX_REFUSE("tcgen05 attention: %d tiles exceed the grid", n_tiles);
     const dim3 grid((unsigned)(n_tiles * n_kv_heads), 1, n_splits);
     if (beside) {
@@ -815,16 +855,16 @@ extern "C" int mx_paged_attention_tc_split(const void* q, int q_stride, const vo
         // the end of what both need (attention_mma.cu): the prompt's tiles then take the SMs that it leaves free, and those
         // that its short requests give back. They wait for it only before they end. 31 requests of up to 6,000 tokens and a
         // portion of 512 (7B sizes, 124 blocks there, 148 here): 2,513 us a step one after the other, 2,473 so.
-        const cudaError_t e = distance ? mx_launch_chained(attention_tc_kernel<true>, grid, dim3(AT_THREADS), smem, stream, q_map, k_map, v_map, p)
-                                       : mx_launch_chained(attention_tc_kernel<false>, grid, dim3(AT_THREADS), smem, stream, q_map, k_map, v_map, p);
+        const cudaError_t e = distance ? mx_launch_chained(attention_tc_kernel<true, false>, grid, dim3(AT_THREADS), smem, stream, q_map, k_map, v_map, p)
+                                       : mx_launch_chained(attention_tc_kernel<false, false>, grid, dim3(AT_THREADS), smem, stream, q_map, k_map, v_map, p);
         if (e != cudaSuccess) {
             mx_set_error("tcgen05 attention: launch failed: %s", cudaGetErrorString(e));
             return (int)e;
         }
         return MX_OK;
     }
-    if (distance) attention_tc_kernel<true><<<grid, AT_THREADS, smem, stream>>>(q_map, k_map, v_map, p);
-    else attention_tc_kernel<false><<<grid, AT_THREADS, smem, stream>>>(q_map, k_map, v_map, p);
+    if (distance) attention_tc_kernel<true, false><<<grid, AT_THREADS, smem, stream>>>(q_map, k_map, v_map, p);
+    else attention_tc_kernel<false, false><<<grid, AT_THREADS, smem, stream>>>(q_map, k_map, v_map, p);
     const int rc = mx_launch_status();
     if (rc != MX_OK || n_splits == 1) return rc;
     return mx_attention_merge_bf16_sink(p.part_o, p.part_ml, out, out_stride, n_tokens, n_heads, AT_HD, n_splits, sink,
@@ -839,4 +879,35 @@ extern "C" int mx_paged_attention_tc(const void* q, int q_stride, const void* ca
     return mx_paged_attention_tc_split(q, q_stride, cache, n_pages, page_size, block_tables, bt_stride, cu_q,
                                        context_lens, tiles, n_tiles, n_tokens, n_heads, n_kv_heads, head_dim, window,
                                        scale, out, out_stride, 1, nullptr, status, 0.f, nullptr, 0, nullptr, 0, stream);
+}
+
+// The keys that groups of sequences have in common, for attention_shared.cu: a tile holds 128 / group tokens of one group.
+// Parts 0 .. n_splits - 1 of `part_o` and `part_ml` (of shared.n_parts a token and head) are written for every token of a group.
+int mx_attention_tc_shared(const void* q, int q_stride, const void* cache, long long n_pages, int page_size,
+                           const int* block_tables, int bt_stride, const int* cu_q, int n_tokens, int n_heads, int n_kv_heads,
+                           int window, float scale, float softcap, int n_tiles, int n_splits, float* part_o, float* part_ml,
+                           const SharedPrefixParams& shared, int* status, cudaStream_t stream) {
+    const int group = n_heads / n_kv_heads;
+    CUtensorMap q_map, k_map, v_map;
+    const int mapped = at_make_maps(&q_map, &k_map, &v_map, q, q_stride, cache, n_pages, page_size, n_tokens, n_kv_heads, group);
+    if (mapped != MX_OK) return mapped;
+    AtParams p = {};
+    p.block_tables = block_tables; p.cu_q = cu_q; p.part_o = part_o; p.part_ml = part_ml; p.n_splits = n_splits;
+    p.status = status; p.n_pages = n_pages; p.n_tiles = n_tiles; p.bt_stride = bt_stride; p.n_heads = n_heads;
+    p.n_kv_heads = n_kv_heads; p.group = group; p.tokens_per_tile = AT_ROWS / group; p.page_size = page_size;
+    p.page_shift = page_size == 16 ? 4 : 5; p.window = window; p.scale_log2 = scale * 1.4426950408889634f;
+    p.cap_log2 = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
+    p.cap_in = softcap > 0.f ? scale / softcap : 0.f;
+    p.shared = shared;
+    const size_t smem = (size_t)(2 + 2 * AT_STAGES * 2) * AT_TILE + 1024;
+    const int reserved = at_reserve<false, true>(smem);
+    if (reserved != MX_OK) return reserved;
+    if ((long long)n_tiles * n_kv_heads > 0x7fffffffLL) MX_REFUSE("tcgen05 attention: %d tiles exceed the grid", n_tiles);
+    const dim3 grid((unsigned)(n_tiles * n_kv_heads), 1, n_splits);
+    const cudaError_t e = mx_launch_chained(attention_tc_kernel<false, true>, grid, dim3(AT_THREADS), smem, stream, q_map, k_map, v_map, p);
+    if (e != cudaSuccess) {
+        mx_set_error("tcgen05 attention: launch failed: %s", cudaGetErrorString(e));
+        return (int)e;
+    }
+    return MX_OK;
 }

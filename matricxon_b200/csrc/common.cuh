@@ -20,6 +20,7 @@
 #define MX_STATUS_BAD_SLOT 2
 #define MX_STATUS_BAD_PAGE 4
 #define MX_STATUS_WAIT_TIMEOUT 8
+#define MX_STATUS_BAD_STEP 16
 
 #define MX_DTYPE_F32 0
 #define MX_DTYPE_BF16 1

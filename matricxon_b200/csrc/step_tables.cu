@@ -1,0 +1,216 @@
+// The metadata of one step, laid out on the GPU from the requests' lengths: positions, sequence numbers and cache slots of
+// its token rows, where each sequence's rows begin, and the block tables its attention reads.
+//
+// Sequence s brings q[s] tokens after context[s] cached ones. Its pages stand in row rows[s] of `tables`, which live on the
+// device from step to step. With pages of P positions it holds have = ceil(context / P) pages and takes
+// need = ceil((context + q) / P) - have more from `free_pages`, in the order of the sequences:
+//   cu_q = running sum of q, base = running sum of need
+//   page(s, k) = tables[shared_rows[s]][k]       k < shared_pages[s]: read through another request's row
+//                tables[rows[s]][k]              k < have
+//                free_pages[base[s] + k - have]  k < have + need; also stored in tables[rows[s]][k]
+//   row cu_q[s] + i: position context + i, slot page(position / P) * P + position % P
+// Entries of the step's block table beyond the last page are -1, and so are those that no query of this step or a later one
+// sees (first_visible_key(context) and the kept first positions, the rule by which the cache manager gives pages back).
+// Rows of the buffers behind the last token get position 0, sequence -1, slot -1. Nothing that the results depend on is
+// changed (lengths, free pages), so a step can be laid out twice.
+//
+// Every block adds up all sequences' lengths for itself (a sequence a thread, 8 to 20 bytes each out of L2), which spares a
+// second launch or a wait between blocks, and then lays out its few sequences. A step that does not fit (more rows than the
+// buffers hold, more pages than there are, a length out of range) sets MX_STATUS_BAD_STEP and every block leaves an empty step:
+// all -1, nothing taken, `tables` as they were.
+// The launch after this one must not begin early: attention kernels read tables and lengths before they wait for what ran
+// before them, so this kernel never lets its successor start (no pdl_trigger).
+#include "common.cuh"
+
+namespace {
+
+constexpr int ST_THREADS = 256;
+constexpr int ST_OWN = 64;              // sequences a block lays out, at most
+constexpr int ST_SLICE = 4096;          // block-table entries of a sequence that one block writes
+
+struct StepTablesParams {
+    const int *q_lens, *context_lens, *rows, *shared_rows, *shared_pages, *free_pages, *n_free;
+    int* tables;
+    int *positions, *tok_seq, *cu_q, *slots, *block_tables, *taken, *status;
+    int n_seqs, n_tokens, n_rows, width, page_size, n_pages, n_free_most, window, keep_first, per_block;
+};
+
+struct Sequence {
+    int q, context, row, shared_row, shared;      // shared: pages
+    int have, need;
+    bool fits;                                    // its numbers are possible
+};
+
+__device__ __forceinline__ Sequence read_sequence(const StepTablesParams& p, int s) {
+    Sequence v;
+    v.q = p.q_lens[s];
+    v.context = p.context_lens[s];
+    v.row = p.rows ? p.rows[s] : s;
+    v.shared_row = p.shared_rows ? p.shared_rows[s] : -1;
+    v.shared = v.shared_row >= 0 ? p.shared_pages[s] : 0;
+    const long long most = (long long)p.width * p.page_size;
+    v.fits = v.q >= 0 && v.context >= 0 && v.row >= -1 && v.row < p.n_rows && v.shared_row < p.n_rows &&
+             (long long)v.context + v.q <= most && (v.row >= 0 || v.q == 0) && v.shared >= 0 &&
+             (long long)v.shared * p.page_size <= v.context;
+    if (!v.fits || v.row < 0) {
+        v.q = v.context = v.shared = 0;
+        v.row = v.shared_row = -1;
+    }
+    v.have = (int)(((long long)v.context + p.page_size - 1) / p.page_size);
+    v.need = (int)(((long long)v.context + v.q + p.page_size - 1) / p.page_size) - v.have;
+    return v;
+}
+
+__global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTablesParams p) {
+    __shared__ long long warp_q[ST_THREADS / 32], warp_need[ST_THREADS / 32];
+    __shared__ long long own_q[ST_OWN], own_need[ST_OWN];
+    __shared__ Sequence own[ST_OWN];
+    __shared__ int repeated[ST_OWN];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int first = blockIdx.x * p.per_block, last = min(p.n_seqs, first + p.per_block);
+    pdl_wait();
+    for (int i = tid; i < ST_OWN; i += ST_THREADS) repeated[i] = 0;
+
+    // ---- running sums over all sequences, a sequence a thread
+    long long q_before = 0, need_before = 0;
+    bool fits = true;
+    for (int s0 = 0; s0 < p.n_seqs; s0 += ST_THREADS) {
+        const int s = s0 + tid;
+        Sequence v = {};
+        v.row = -1;
+        v.fits = true;
+        if (s < p.n_seqs) v = read_sequence(p, s);
+        fits = fits && v.fits;
+        long long q = v.q, need = v.need;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long a = __shfl_up_sync(0xffffffffu, q, o), b = __shfl_up_sync(0xffffffffu, need, o);
+            if (lane >= o) { q += a; need += b; }
+        }
+        if (lane == 31) { warp_q[warp] = q; warp_need[warp] = need; }
+        __syncthreads();
+        long long q_all = 0, need_all = 0;
+#pragma unroll
+        for (int w = 0; w < ST_THREADS / 32; ++w) {
+            if (w == warp) { q += q_all; need += need_all; }
+            q_all += warp_q[w];
+            need_all += warp_need[w];
+        }
+        if (s >= first && s < last) {
+            own[s - first] = v;
+            own_q[s - first] = q_before + q - v.q;
+            own_need[s - first] = need_before + need - v.need;
+        }
+        q_before += q_all;
+        need_before += need_all;
+        __syncthreads();
+    }
+    const int n_free = min(*p.n_free, p.n_free_most);
+    const bool possible = __syncthreads_and(fits) && q_before <= p.n_tokens && need_before <= n_free;
+    const int total = possible ? (int)q_before : 0;
+    // a row that an earlier sequence has already: the later one is laid out as empty
+    if (possible && p.rows) {
+        for (int s = tid; s < last; s += ST_THREADS) {
+            const int row = p.rows[s];
+            if (row < 0) continue;
+            for (int i = max(first, s + 1); i < last; ++i)
+                if (own[i - first].row == row) repeated[i - first] = 1;
+        }
+        __syncthreads();
+    }
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) {
+        p.cu_q[0] = 0;
+        *p.taken = possible ? (int)need_before : 0;
+        if (!possible) atomicOr(p.status, MX_STATUS_BAD_STEP);
+    }
+
+    // ---- this block's sequences
+    const int k_begin = blockIdx.y * ST_SLICE, k_end = min(p.width, k_begin + ST_SLICE);
+    for (int s = first; s < last; ++s) {
+        const Sequence v = own[s - first];
+        const int begin = (int)own_q[s - first], taken = (int)own_need[s - first];
+        const bool there = possible && v.row >= 0 && !repeated[s - first];
+        if (blockIdx.y == 0 && tid == 0) {
+            p.cu_q[s + 1] = possible ? begin + v.q : 0;
+            if (possible && repeated[s - first]) atomicOr(p.status, MX_STATUS_BAD_STEP);
+        }
+        int* mine = p.tables + (size_t)max(v.row, 0) * p.width;
+        const int* leader = p.tables + (size_t)max(v.shared_row, 0) * p.width;
+        const int end = there ? v.have + v.need : 0;
+        // pages that nobody sees any more: between the kept ones and the first that the next query needs
+        const int kept = p.window > 0 ? (p.keep_first + p.page_size - 1) / p.page_size : 0;
+        const int seen_from = first_visible_key(v.context, p.window) / p.page_size;
+        int* out = p.block_tables + (size_t)s * p.width;
+        bool bad_page = false;
+#pragma unroll 4
+        for (int k = k_begin + tid; k < k_end; k += ST_THREADS) {
+            int page = -1;
+            if (k < end) {
+                const bool is_new = k >= v.have;
+                page = is_new ? p.free_pages[taken + k - v.have] : (k < v.shared ? leader[k] : mine[k]);
+                const bool seen = k < kept || k >= seen_from;
+                if (is_new) mine[k] = page;
+                if (!seen) page = -1;
+                else if (page < 0 || page >= p.n_pages) {
+                    page = -1;
+                    bad_page = true;
+                }
+            }
+            out[k] = page;
+        }
+        if (bad_page) atomicOr(p.status, MX_STATUS_BAD_PAGE);
+        if (blockIdx.y == 0 && possible) {
+            for (int i = tid; i < v.q; i += ST_THREADS) {
+                const int position = v.context + i, k = position / p.page_size;
+                int slot = -1;
+                if (there) {
+                    const int page = k >= v.have ? p.free_pages[taken + k - v.have] : mine[k];
+                    if (page >= 0 && page < p.n_pages) slot = page * p.page_size + position % p.page_size;
+                    else atomicOr(p.status, MX_STATUS_BAD_PAGE);
+                }
+                p.positions[begin + i] = there ? position : 0;
+                p.tok_seq[begin + i] = there ? s : -1;
+                p.slots[begin + i] = slot;
+            }
+        }
+    }
+    // ---- rows behind the last token
+    if (blockIdx.y == 0)
+        for (int t = total + blockIdx.x * ST_THREADS + tid; t < p.n_tokens; t += gridDim.x * ST_THREADS) {
+            p.positions[t] = 0;
+            p.tok_seq[t] = -1;
+            p.slots[t] = -1;
+        }
+}
+
+}  // namespace
+
+extern "C" int mx_step_tables(const int* q_lens, const int* context_lens, const int* rows, int n_seqs, int* tables, int n_rows,
+                              int width, const int* free_pages, int n_free_most, const int* n_free, int page_size,
+                              long long n_pages, const int* shared_rows, const int* shared_pages, int window, int keep_first,
+                              int* positions, int* tok_seq, int* cu_q, int* slots, int n_tokens, int* block_tables, int* taken,
+                              int* status, cudaStream_t stream) {
+    if (n_seqs <= 0) MX_REFUSE("step tables: a step of %d sequences", n_seqs);
+    if (width <= 0 || n_rows <= 0 || n_tokens < 0) MX_REFUSE("step tables: %d rows of %d entries, %d tokens", n_rows, width, n_tokens);
+    if (page_size <= 0) MX_REFUSE("step tables: pages of %d positions", page_size);
+    if (n_pages <= 0 || n_pages * page_size > 0x7fffffffLL) MX_REFUSE("step tables: %lld pages of %d positions have no 32-bit slots", n_pages, page_size);
+    if (keep_first < 0) MX_REFUSE("step tables: %d kept positions", keep_first);
+    if ((shared_rows == nullptr) != (shared_pages == nullptr)) MX_REFUSE("step tables: shared rows and shared pages go together");
+    StepTablesParams p;
+    p.q_lens = q_lens; p.context_lens = context_lens; p.rows = rows; p.shared_rows = shared_rows; p.shared_pages = shared_pages;
+    p.free_pages = free_pages; p.n_free = n_free; p.tables = tables; p.positions = positions; p.tok_seq = tok_seq; p.cu_q = cu_q;
+    p.slots = slots; p.block_tables = block_tables; p.taken = taken; p.status = status;
+    p.n_seqs = n_seqs; p.n_tokens = n_tokens; p.n_rows = n_rows; p.width = width; p.page_size = page_size; p.n_pages = (int)n_pages;
+    p.n_free_most = n_free_most; p.window = window; p.keep_first = window > 0 ? keep_first : 0;
+    // a block a sequence while that makes no more than four blocks an SM
+    p.per_block = (n_seqs + 591) / 592;
+    if (p.per_block > ST_OWN) MX_REFUSE("step tables: %d sequences, at most %d a step", n_seqs, 592 * ST_OWN);
+    const dim3 grid((n_seqs + p.per_block - 1) / p.per_block, (width + ST_SLICE - 1) / ST_SLICE);
+    if (grid.y > 65535) MX_REFUSE("step tables: tables of %d entries a row", width);
+    const cudaError_t e = mx_launch_chained(step_tables_kernel, grid, dim3(ST_THREADS), 0, stream, p);
+    if (e != cudaSuccess) {
+        mx_set_error("step tables: launch failed: %s", cudaGetErrorString(e));
+        return (int)e;
+    }
+    return MX_OK;
+}

@@ -25,7 +25,8 @@ def _launched(n: int = 1) -> None:
 
 
 STATUS_BITS = {1: "a token id outside the vocabulary", 2: "a cache slot outside the pool",
-               4: "a block-table entry that names no page", 8: "a device-side wait ran out"}
+               4: "a block-table entry that names no page", 8: "a device-side wait ran out",
+               16: "a step that does not fit the rows, pages or tables it was given"}
 
 
 def dtype_code(dtype: torch.dtype) -> int:
@@ -665,6 +666,205 @@ def paged_attention_mma(q: torch.Tensor, q_stride: int, cache: torch.Tensor,
 def mma_attention_supported(dtype: torch.dtype, head_dim: int, page_size: int, q_stride: int) -> bool:
     return (dtype == torch.bfloat16 and head_dim in (64, 128) and page_size in (8, 16, 32)
             and q_stride % 8 == 0)
+
+
+def _need_here(*tensors: tuple[str, torch.Tensor | None]) -> None:
+    """Launches go to the current device's current stream: tensors of another device are refused."""
+    here = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for name, tensor in tensors:
+        if tensor is None:
+            continue
+        if not tensor.is_cuda:
+            raise KernelLibraryError(f"{name} must be a CUDA tensor (there is no CPU path)")
+        if tensor.device.index != here or (_device_index is not None and here != _device_index):
+            raise KernelLibraryError(f"{name} is on {tensor.device}, kernels run on cuda:{here if _device_index is None else _device_index}")
+
+
+def _need_ints(name: str, tensor: torch.Tensor | None, *shape: int) -> None:
+    """``tensor`` (where there is one): contiguous int32 of that shape, -1 for any size."""
+    if tensor is None:
+        return
+    _need(tensor, name, torch.int32)
+    if tensor.ndim != len(shape) or any(want >= 0 and have != want for have, want in zip(tensor.shape, shape)):
+        raise KernelLibraryError(f"{name} must be int32 {list(shape)}, got {list(tensor.shape)}")
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_shared_scratch(*sizes: int) -> int:
+    return int(library().mx_attention_shared_scratch(*sizes))
+
+
+def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, block_tables: torch.Tensor,
+                           cu_q: torch.Tensor, context_lens: torch.Tensor, tok_seq: torch.Tensor, positions: torch.Tensor,
+                           shared_first: torch.Tensor, shared_lens: torch.Tensor, n_tokens: int, n_heads: int,
+                           n_kv_heads: int, head_dim: int, window: int | None, scale: float, out: torch.Tensor,
+                           status: torch.Tensor, *, max_q_len: int, max_shared_len: int, max_own_len: int,
+                           softcap: float | None = None, sink: torch.Tensor | None = None,
+                           scratch: torch.Tensor | None = None) -> None:
+    """Attention of a step whose sequences lie in groups that have their first keys in common, which are read once for
+    a whole group (float32 or bfloat16, any head size ``paged_attention`` takes).
+
+    Sequences ``shared_first[g] .. shared_first[g + 1] - 1`` (int32 [groups + 1], from 0 to the number of sequences) are
+    group g. Sequence s reads its keys below ``shared_lens[s]`` (int32, one per sequence; 0: none) through the block table
+    of its group's first sequence, the others through its own, so the tables of ``paged_attention`` serve as they are: shared
+    pages stand in every table of the group. ``q``, ``out``, ``window``, ``softcap`` and ``sink`` as in ``paged_attention``;
+    sequence s brings rows ``cu_q[s] .. cu_q[s + 1] - 1``, row i of it at position ``context_lens[s] + i``, which
+    ``positions`` and ``tok_seq`` repeat row by row. Rows from ``cu_q[-1]`` on are left alone.
+
+    ``max_q_len``: no sequence brings more tokens (one that does sets the status word). ``max_shared_len``,
+    ``max_own_len`` (keys that a sequence shares, and does not) are for sizing: with other numbers the result is the same
+    up to rounding. All three are host numbers, so that a captured step can be replayed with other lengths and groups
+    below them. ``scratch`` (float32) is taken from torch's allocator where none is given. The keys and values that any
+    token of a group sees have to be finite."""
+    _need(q, "q", contiguous=False)
+    _need(cache, "cache", q.dtype)
+    _need(out, "out", q.dtype, contiguous=False)
+    _need_here(("q", q), ("cache", cache), ("block_tables", block_tables), ("cu_q", cu_q), ("context_lens", context_lens),
+               ("tok_seq", tok_seq), ("positions", positions), ("shared_first", shared_first), ("shared_lens", shared_lens),
+               ("out", out), ("status", status), ("sink", sink), ("scratch", scratch))
+    code = dtype_code(q.dtype)
+    n_seqs = context_lens.numel()
+    for name, tensor, shape in (("context_lens", context_lens, (n_seqs,)), ("block_tables", block_tables, (n_seqs, -1)),
+                                ("cu_q", cu_q, (n_seqs + 1,)), ("tok_seq", tok_seq, (-1,)), ("positions", positions, (-1,)),
+                                ("shared_first", shared_first, (-1,)), ("shared_lens", shared_lens, (n_seqs,))):
+        _need_ints(name, tensor, *shape)
+    _need(status, "status", torch.int32)
+    n_groups = shared_first.numel() - 1
+    if n_groups < 1 and n_seqs > 0:
+        raise KernelLibraryError("shared_first must hold the start of at least one group and the end of the last")
+    page_size = cache.shape[3] if cache.ndim == 5 else 0
+    if tuple(cache.shape[1:]) != (2, n_kv_heads, page_size, head_dim):
+        raise KernelLibraryError(f"cache must be [pages, 2, {n_kv_heads}, page size, {head_dim}], got {list(cache.shape)}")
+    if min(tok_seq.numel(), positions.numel()) < n_tokens or q.ndim != 2 or q.shape[0] < n_tokens:
+        raise KernelLibraryError(f"q, tok_seq and positions must hold {n_tokens} rows")
+    if q.stride(1) != 1 or q_stride != q.stride(0) or q.shape[1] < n_heads * head_dim:
+        raise KernelLibraryError(f"q must hold rows of {n_heads * head_dim} numbers, q_stride apart, got {list(q.shape)}")
+    if out.ndim != 2 or out.shape[0] < n_tokens or out.shape[1] != n_heads * head_dim or out.stride(1) != 1:
+        raise KernelLibraryError(f"out must hold {n_tokens} rows of {n_heads * head_dim} numbers, got {list(out.shape)}")
+    if n_tokens <= 0 or n_seqs == 0:
+        return
+    aligned = q_stride % 8 == 0 and q.data_ptr() % 16 == 0 and cache.data_ptr() % 16 == 0
+    n_sm = sm_count(q.device)
+    need = _attention_shared_scratch(code, int(aligned), page_size, n_seqs, n_groups, n_tokens, n_heads, n_kv_heads, head_dim,
+                                     int(max_q_len), int(max_shared_len), int(max_own_len), n_sm)
+    if scratch is None:
+        scratch = torch.empty((need + 3) // 4, dtype=torch.float32, device=q.device)
+    _need(scratch, "scratch", torch.float32)
+    if scratch.numel() * 4 < need or scratch.data_ptr() % 16 != 0:
+        raise KernelLibraryError(f"attention over shared keys needs {need} bytes of 16-byte aligned scratch")
+    check(library().mx_paged_attention_shared(
+        _ptr(q), code, q_stride, _ptr(cache), cache.shape[0], page_size, _ptr(block_tables), block_tables.stride(0),
+        _ptr(cu_q), _ptr(context_lens), _ptr(tok_seq), _ptr(positions), _ptr(shared_first), _ptr(shared_lens), n_seqs,
+        n_groups, n_tokens, n_heads, n_kv_heads, head_dim, int(window or 0), float(scale), float(softcap or 0.0),
+        _sink_ptr(sink, n_heads), _ptr(out), out.stride(0), int(max_q_len), int(max_shared_len), int(max_own_len), n_sm,
+        _ptr(scratch), _ptr(status), _stream()), "paged_attention_shared")
+    _launched(3 if max_shared_len > 0 else 2)
+
+
+# ---------------------------------------------------------------------- a step's metadata
+def step_tables(q_lens: torch.Tensor, context_lens: torch.Tensor, rows: torch.Tensor | None, tables: torch.Tensor,
+                free_pages: torch.Tensor, n_free: torch.Tensor, page_size: int, n_pages: int, positions: torch.Tensor,
+                tok_seq: torch.Tensor, cu_q: torch.Tensor, slots: torch.Tensor, block_tables: torch.Tensor,
+                taken: torch.Tensor, status: torch.Tensor, *, shared_rows: torch.Tensor | None = None,
+                shared_pages: torch.Tensor | None = None, window: int | None = None, keep_first: int = 0) -> None:
+    """Lays a step's metadata out on the GPU from the requests' lengths, in one launch (everything int32).
+
+    Sequence s brings ``q_lens[s]`` tokens after ``context_lens[s]`` cached ones; its pages stand in row ``rows[s]`` of
+    ``tables`` [table rows, width] (``rows`` None: row s; -1: a padding sequence, which brings nothing). The pages it needs
+    beyond those it holds are the next ones of ``free_pages``, in the order of the sequences, and are stored in its row;
+    ``n_free`` [1] says how many of them there are, ``taken`` [1] how many the step took. Where ``shared_rows[s]`` >= 0 its first
+    ``shared_pages[s]`` pages, all full, are read from that row instead.
+
+    Written: ``cu_q`` [sequences + 1], ``positions``, ``tok_seq`` and cache ``slots`` of every token row (rows behind the last
+    token: 0, -1, -1) and ``block_tables`` [sequences, width], -1 where there is no page or none that a query from
+    ``context_lens[s]`` on sees: ``window`` and ``keep_first`` as in ``paged_attention``, a negative window for blocks. Lengths and
+    free pages are only read, so the same step may be laid out again. A step that does not fit sets the status word and
+    comes out empty, with ``tables`` as they were; of two sequences with one row the later one does."""
+    tensors = (("q_lens", q_lens), ("context_lens", context_lens), ("rows", rows), ("tables", tables), ("free_pages", free_pages),
+               ("n_free", n_free), ("positions", positions), ("tok_seq", tok_seq), ("cu_q", cu_q), ("slots", slots),
+               ("block_tables", block_tables), ("taken", taken), ("status", status), ("shared_rows", shared_rows),
+               ("shared_pages", shared_pages))
+    _need_here(*tensors)
+    n_seqs, n_tokens = q_lens.numel(), positions.numel()
+    width = tables.shape[-1]
+    shapes = {"q_lens": (n_seqs,), "context_lens": (n_seqs,), "rows": (n_seqs,), "tables": (-1, -1), "free_pages": (-1,),
+              "n_free": (1,), "positions": (-1,), "tok_seq": (n_tokens,), "cu_q": (n_seqs + 1,), "slots": (n_tokens,),
+              "block_tables": (n_seqs, width), "taken": (1,), "status": (1,), "shared_rows": (n_seqs,), "shared_pages": (n_seqs,)}
+    for name, tensor in tensors:
+        _need_ints(name, tensor, *shapes[name])
+    if rows is None and tables.shape[0] < n_seqs:
+        raise KernelLibraryError(f"{n_seqs} sequences need as many rows of tables, got {tables.shape[0]}")
+    check(library().mx_step_tables(
+        _ptr(q_lens), _ptr(context_lens), _ptr(rows), n_seqs, _ptr(tables), tables.shape[0], width, _ptr(free_pages),
+        free_pages.numel(), _ptr(n_free), int(page_size), int(n_pages), _ptr(shared_rows), _ptr(shared_pages), int(window or 0),
+        int(keep_first), _ptr(positions), _ptr(tok_seq), _ptr(cu_q), _ptr(slots), n_tokens, _ptr(block_tables), _ptr(taken),
+        _ptr(status), _stream()), "step_tables")
+    _launched()
+
+
+# ---------------------------------------------------------------------- scores before a token is drawn
+def adjust_logits(logits: torch.Tensor, out: torch.Tensor, token_offsets: torch.Tensor | None = None,
+                  token_ids: torch.Tensor | None = None, repeat_penalty: torch.Tensor | None = None,
+                  presence_penalty: torch.Tensor | None = None, frequency_penalty: torch.Tensor | None = None, *,
+                  bias_offsets: torch.Tensor | None = None, bias_ids: torch.Tensor | None = None,
+                  bias_values: torch.Tensor | None = None, mask_words: torch.Tensor | None = None,
+                  mask_rows: torch.Tensor | None = None, pending_ids: torch.Tensor | None = None) -> None:
+    """``out`` (float32 [rows, vocab], may be ``logits`` itself) <- the scores of ``logits`` (float32 or bfloat16) with each
+    row's penalties, biases and mask.
+
+    ``token_ids[token_offsets[r]:token_offsets[r + 1]]`` (int32) are the ids row r has generated, in any order and as often as
+    they came; ``pending_ids`` [rows] one more each (-1: none). A token among them, c times, has its score divided (positive)
+    or multiplied (negative) by ``repeat_penalty[r]`` and then loses ``frequency_penalty[r] * c + presence_penalty[r]``
+    (float32 [rows]). ``bias_values`` (float32) are added at ``bias_ids``, row r's at ``bias_offsets[r]:bias_offsets[r + 1]``; of
+    two of one token the later one counts. ``mask_words`` (int32 [masks, words]): bit v % 32 of word v / 32 says whether
+    token v may be taken; a score that may not becomes -infinity. Row r goes by mask ``mask_rows[r]`` (-1: none), or by
+    mask r where there is no ``mask_rows``. Ids outside the vocabulary are passed over. Rows of ``logits`` and ``out`` may be
+    strided."""
+    tensors = (("token_offsets", token_offsets), ("token_ids", token_ids), ("bias_offsets", bias_offsets), ("bias_ids", bias_ids),
+               ("mask_words", mask_words), ("mask_rows", mask_rows), ("pending_ids", pending_ids))
+    floats = (("repeat_penalty", repeat_penalty), ("presence_penalty", presence_penalty), ("frequency_penalty", frequency_penalty),
+              ("bias_values", bias_values))
+    _need(logits, "logits", contiguous=False)
+    _need(out, "out", torch.float32, contiguous=False)
+    _need_here(("logits", logits), ("out", out), *tensors, *floats)
+    code = dtype_code(logits.dtype)
+    if logits.ndim != 2 or logits.shape != out.shape or logits.stride(1) != 1 or out.stride(1) != 1:
+        raise KernelLibraryError(f"logits and out must be [rows, vocab] with neighbouring columns, got {list(logits.shape)} and {list(out.shape)}")
+    n_rows, vocab = logits.shape
+    if n_rows > 1 and out.stride(0) < vocab:
+        raise KernelLibraryError("rows of out must not overlap")
+    shapes = {"token_offsets": (n_rows + 1,), "token_ids": (-1,), "bias_offsets": (n_rows + 1,), "bias_ids": (-1,),
+              "mask_words": (-1, -1), "mask_rows": (n_rows,), "pending_ids": (n_rows,)}
+    for name, tensor in tensors:
+        _need_ints(name, tensor, *shapes[name])
+    for name, tensor in floats:
+        if tensor is not None:
+            _need(tensor, name, torch.float32)
+            if name != "bias_values" and tensor.shape != (n_rows,):
+                raise KernelLibraryError(f"{name} must be float32 [{n_rows}], got {list(tensor.shape)}")
+    if (token_offsets is None) != (token_ids is None):
+        raise KernelLibraryError("token_offsets and token_ids go together")
+    if len({bias_offsets is None, bias_ids is None, bias_values is None}) > 1 or (
+            bias_ids is not None and bias_ids.shape != bias_values.shape):
+        raise KernelLibraryError("bias_offsets, bias_ids and bias_values go together, a value an id")
+    if mask_words is None and mask_rows is not None or mask_words is not None and mask_rows is None and mask_words.shape[0] != n_rows:
+        raise KernelLibraryError("mask_rows says which of mask_words' rows a row of scores goes by; without it there is one each")
+    if n_rows == 0:
+        return
+    first, last = logits.data_ptr(), logits.data_ptr() + ((n_rows - 1) * logits.stride(0) + vocab) * logits.element_size()
+    if first < out.data_ptr() + ((n_rows - 1) * out.stride(0) + vocab) * 4 and out.data_ptr() < last:
+        # the same rows, or other columns of the same buffer
+        stride = out.stride(0)
+        apart = (out.data_ptr() - first) // 4 % max(stride, 1)
+        if code != F32 or n_rows > 1 and stride != logits.stride(0) or not (
+                out.data_ptr() == first or n_rows > 1 and vocab <= apart <= stride - vocab):
+            raise KernelLibraryError("out lies over a part of logits; it may be the same rows, or others")
+    check(library().mx_adjust_logits(
+        _ptr(logits), code, logits.stride(0), _ptr(out), out.stride(0), n_rows, vocab, _ptr(token_offsets), _ptr(token_ids),
+        _ptr(repeat_penalty), _ptr(presence_penalty), _ptr(frequency_penalty), _ptr(bias_offsets), _ptr(bias_ids), _ptr(bias_values),
+        _ptr(mask_words), 0 if mask_words is None else mask_words.shape[0], 0 if mask_words is None else mask_words.shape[1],
+        _ptr(mask_rows), _ptr(pending_ids), _stream()), "adjust_logits")
+    _launched()
 
 
 # ---------------------------------------------------------------------- RMS norm, post-norm sums
