@@ -8,86 +8,309 @@
 // in float, from float or bfloat16 scores. An id outside the vocabulary counts for nothing; of a token with two biases the
 // later one holds; a row without a mask (mask_rows < 0) may take every token.
 //
-// A block owns a stretch of one row's vocabulary. It keeps, in shared memory, a word a token of its stretch: the count, and
-// which entry of the bias list is the token's (largest index first). The row's ids are read whole by each of the row's blocks,
-// which needs no sorting, no scratch memory and no second launch; integer atomics in shared memory make the counts
-// independent of the order. Scores that the mask shuts out are not read.
+// A block owns a stretch of one row's vocabulary. It first writes the scores as the mask leaves them, which is bound by memory:
+// fours as 16-byte accesses wherever the rows of both sides lie alike (stretches are counted from the 16-byte boundary before
+// the row, so odd vocabularies do); a four is asked for a turn before it is written, its mask a turn before that, and not
+// at all if the mask shuts it out. Nothing in that loop may branch on a score: a look at each score's count there made it three
+// times as long. Then the block counts, in shared memory, how often each token of its stretch stands in the row's list, and
+// deals with each of them once, in what it has just written: of the threads that have one of a token's places the first to
+// take its count does so. Integer atomics: the order in which threads come does not matter. The biases come last, the largest
+// place in the list among a token's biases says which one holds. What a phase reads it asks for eight at a time.
+// Where a row has many blocks and a long list, a kernel beside deals the ids out to the stretches first, so that each is looked
+// at once, not by every block of the row.
+// 256 rows of 131,071 scores, a third of them allowed, with 6,144 ids each: 90 us, 121 with every block reading the whole list (a copy of
+// such scores takes 47).
 #include <math.h>
 
 #include "common.cuh"
+#include "shared_prefix.cuh"
 
 namespace {
 
-constexpr int AL_THREADS = 256;
+constexpr int AL_THREADS = 256, AL_FOURS = 2;        // fours of scores a thread has on their way
+constexpr int AL_TURN = 4 * AL_FOURS * AL_THREADS;
+constexpr int AL_AHEAD = 8;                          // ids a thread asks for at a time
+constexpr int DEAL_THREADS = 512;
+constexpr int DEAL_BLOCKS = 1024;                    // stretches of a row that ids are dealt out to, at most
 
 struct AdjustParams {
     const void* logits;
     float* out;
     long long row_stride, out_stride;
-    int vocab, stretch, mask_width, n_masks;
+    int vocab, mask_width, n_masks;
     const int *token_offsets, *token_ids, *bias_offsets, *bias_ids, *mask_words, *mask_rows, *pending;
     const float *repeat, *presence, *frequency, *bias_values;
+    int stretch;                                     // scores of a block
+    int *dealt, *dealt_from;                         // ids by stretch, and where each stretch's begin [rows][blocks + 1]; or null
 };
 
-template <typename T>
-__global__ void __launch_bounds__(AL_THREADS) adjust_logits_kernel(const AdjustParams p) {
-    extern __shared__ int words[];
-    const int row = blockIdx.y, tid = threadIdx.x;
-    const int begin = blockIdx.x * p.stretch, n = min(p.stretch, p.vocab - begin);
-    pdl_trigger();
+__device__ __forceinline__ const unsigned* mask_of(const AdjustParams& p, int row) {
+    if (p.mask_words == nullptr) return nullptr;
+    const int at = p.mask_rows ? p.mask_rows[row] : row;
+    return at >= 0 && at < p.n_masks ? reinterpret_cast<const unsigned*>(p.mask_words) + (size_t)at * p.mask_width : nullptr;
+}
+
+__device__ __forceinline__ void load_four(const float* from, float* x) {
+    const float4 v = *reinterpret_cast<const float4*>(from);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+__device__ __forceinline__ void load_four(const __nv_bfloat16* from, float* x) {
+    const uint2 v = *reinterpret_cast<const uint2*>(from);
+    x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
+    x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+}
+
+// Tokens are counted from the 16-byte boundary before the row's first one: place j is token j - shift.
+__device__ __forceinline__ int shift_of(const AdjustParams& p, int row) {
+    return (int)(reinterpret_cast<uintptr_t>(p.out + (size_t)row * p.out_stride) >> 2 & 3);
+}
+
+// A row's ids (and the pending one) sorted by stretch, in any order within one: counted, then put in place. A block a row.
+__global__ void __launch_bounds__(DEAL_THREADS) deal_ids_kernel(const AdjustParams p, int n_blocks) {
+    __shared__ int count[DEAL_BLOCKS];
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
     pdl_wait();
-    int* counts = words;
-    int* bias_at = words + p.stretch;
+    pdl_trigger();                                    // the scores' kernel begins beside this one
     const int first = p.token_offsets ? p.token_offsets[row] : 0, last = p.token_offsets ? p.token_offsets[row + 1] : 0;
-    const int pending = p.pending ? p.pending[row] : -1;
-    const int bias_first = p.bias_offsets ? p.bias_offsets[row] : 0, bias_last = p.bias_offsets ? p.bias_offsets[row + 1] : 0;
-    const int mask_row = p.mask_rows ? p.mask_rows[row] : (p.mask_words ? row : -1);
-    const bool counted = last > first || pending >= 0, biased = bias_last > bias_first;
-    const int* mask = mask_row >= 0 && mask_row < p.n_masks ? p.mask_words + (size_t)mask_row * p.mask_width : nullptr;
-    if (counted)
-        for (int i = tid; i < n; i += AL_THREADS) counts[i] = 0;
-    if (biased)
-        for (int i = tid; i < n; i += AL_THREADS) bias_at[i] = -1;
-    if (counted || biased) __syncthreads();
-    if (counted) {
-        for (int j = first + tid; j < last; j += AL_THREADS) {
-            const unsigned at = (unsigned)(p.token_ids[j] - begin);
-            if (at < (unsigned)n) atomicAdd(&counts[at], 1);
+    const int pending = p.pending ? p.pending[row] : -1, shift = shift_of(p, row);
+    const int n = max(last - first, 0) + 1;
+    // the stretches of ids k0 + tid, + DEAL_THREADS, ... (-1: none)
+    auto ahead = [&](int k0, int* id, int* to) {
+#pragma unroll
+        for (int e = 0; e < AL_AHEAD; ++e) {
+            const int k = k0 + e * DEAL_THREADS + tid;
+            id[e] = k >= n ? -1 : (k == n - 1 ? pending : p.token_ids[first + k]);
         }
-        if (tid == 0 && pending >= begin && pending < begin + n) atomicAdd(&counts[pending - begin], 1);
+#pragma unroll
+        for (int e = 0; e < AL_AHEAD; ++e) to[e] = id[e] >= 0 && id[e] < p.vocab ? (id[e] + shift) / p.stretch : -1;
+    };
+    int id[AL_AHEAD], to[AL_AHEAD];
+    for (int i = tid; i < n_blocks; i += DEAL_THREADS) count[i] = 0;
+    __syncthreads();
+    for (int k0 = 0; k0 < n; k0 += AL_AHEAD * DEAL_THREADS) {
+        ahead(k0, id, to);
+#pragma unroll
+        for (int e = 0; e < AL_AHEAD; ++e)
+            if (to[e] >= 0) atomicAdd(&count[to[e]], 1);
     }
-    if (biased)
-        for (int j = bias_first + tid; j < bias_last; j += AL_THREADS) {
-            const unsigned at = (unsigned)(p.bias_ids[j] - begin);
-            if (at < (unsigned)n) atomicMax(&bias_at[at], j);
-        }
-    if (counted || biased) __syncthreads();
-    const float repeat = p.repeat ? p.repeat[row] : 1.f, presence = p.presence ? p.presence[row] : 0.f;
-    const float frequency = p.frequency ? p.frequency[row] : 0.f;
-    const T* src = reinterpret_cast<const T*>(p.logits) + (size_t)row * p.row_stride + begin;
-    float* dst = p.out + (size_t)row * p.out_stride + begin;
-#pragma unroll 4
-    for (int i = tid; i < n; i += AL_THREADS) {
-        const int v = begin + i;
-        const bool allowed = mask == nullptr || ((unsigned)mask[v >> 5] >> (v & 31) & 1u);
-        float x = allowed ? to_float(src[i]) : -INFINITY;
-        if (allowed) {
-            const int c = counted ? counts[i] : 0;
-            if (c > 0) {
-                x = x > 0.f ? x / repeat : x * repeat;
-                x -= frequency * (float)c + presence;
+    __syncthreads();
+    if (tid < 32) {
+        int before = 0;
+        for (int i0 = 0; i0 < n_blocks; i0 += 32) {
+            const int i = i0 + lane, mine = i < n_blocks ? count[i] : 0;
+            int through = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, through, o);
+                if (lane >= o) through += up;
             }
-            if (biased && bias_at[i] >= 0) x += p.bias_values[bias_at[i]];
+            if (i < n_blocks) {
+                count[i] = before + through - mine;
+                p.dealt_from[(size_t)row * (n_blocks + 1) + i] = before + through - mine;
+            }
+            before += __shfl_sync(0xffffffffu, through, 31);
         }
-        dst[i] = x;
+        if (lane == 0) p.dealt_from[(size_t)row * (n_blocks + 1) + n_blocks] = before;
+    }
+    __syncthreads();
+    int* dealt = p.dealt + (size_t)first + row;       // behind the lists before this one, and a pending id each
+    for (int k0 = 0; k0 < n; k0 += AL_AHEAD * DEAL_THREADS) {    // the same trips for every lane
+        ahead(k0, id, to);
+#pragma unroll
+        for (int e = 0; e < AL_AHEAD; ++e) {
+            // most ids are frequent tokens, of one stretch: its lanes take their places together
+            const unsigned peers = __match_any_sync(0xffffffffu, to[e]);
+            const int leader = __ffs(peers) - 1;
+            int at = 0;
+            if (to[e] >= 0 && lane == leader) at = atomicAdd(&count[to[e]], __popc(peers));
+            at = __shfl_sync(0xffffffffu, at, leader) + __popc(peers & ((1u << lane) - 1u));
+            if (to[e] >= 0) dealt[at] = id[e];
+        }
     }
 }
 
 template <typename T>
-int launch_adjust(const AdjustParams& p, int n_rows, cudaStream_t stream) {
-    const size_t smem = (size_t)p.stretch * 8;
-    const dim3 grid((p.vocab + p.stretch - 1) / p.stretch, n_rows);
-    const cudaError_t e = mx_launch_chained(adjust_logits_kernel<T>, grid, dim3(AL_THREADS), smem, stream, p);
+__global__ void __launch_bounds__(AL_THREADS, 5) adjust_logits_kernel(const AdjustParams p) {
+    extern __shared__ __align__(16) int words[];      // a word a token of the stretch
+    const int row = blockIdx.y, tid = threadIdx.x;
+    if (p.dealt == nullptr) pdl_wait();               // the kernel before this one has waited otherwise
+    const T* src = reinterpret_cast<const T*>(p.logits) + (size_t)row * p.row_stride;
+    float* dst = p.out + (size_t)row * p.out_stride;
+    const unsigned* mask = mask_of(p, row);
+    const int shift = shift_of(p, row);
+    const bool alike = (reinterpret_cast<uintptr_t>(src - shift) & (4 * sizeof(T) - 1)) == 0;
+    const int begin = (int)min((long long)blockIdx.x * p.stretch, (long long)p.vocab + shift);
+    const int end = min(begin + p.stretch, p.vocab + shift);
+    // The fours that lie wholly in the row: places from `low` to `high`. What is left, up to three tokens at either end of the
+    // row, is done one by one.
+    const int row_low = (shift + 3) & ~3, row_high = (p.vocab + shift) & ~3;
+    const int low = max(begin, row_low), high = min(end, row_high);
+    auto takes = [&](int v) { return mask == nullptr || (mask[v >> 5] >> (v & 31) & 1u); };
+    // which tokens of the four at place j the row may take (a bit each), and their scores if there are any
+    auto bits_at = [&](int j) -> unsigned {
+        if (j >= high) return 0u;
+        if (mask == nullptr) return 15u;
+        const int v = j - shift;
+        const unsigned* word = mask + (v >> 5);
+        // the four lies in two words only where the row is shifted against the mask
+        const unsigned more = shift != 0 && (v & 31) > 28 ? word[1] : 0u;
+        return __funnelshift_r(word[0], more, v & 31) & 15u;
+    };
+    auto load = [&](int j, unsigned allowed, float* x) {
+        if (allowed == 0) return;
+        const T* from = src + (j - shift);
+        if (alike) {
+            load_four(from, x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = to_float(from[e]);
+        }
+    };
+    float next[AL_FOURS][4];
+    unsigned next_bits[AL_FOURS], later_bits[AL_FOURS];
+#pragma unroll
+    for (int u = 0; u < AL_FOURS; ++u) next_bits[u] = bits_at(low + 4 * (tid + u * AL_THREADS));
+#pragma unroll
+    for (int u = 0; u < AL_FOURS; ++u) {
+        load(low + 4 * (tid + u * AL_THREADS), next_bits[u], next[u]);
+        later_bits[u] = bits_at(low + 4 * (tid + u * AL_THREADS) + AL_TURN);
+    }
+    for (int j0 = low + 4 * tid; j0 < high; j0 += AL_TURN) {
+        float x[AL_FOURS][4];
+        unsigned allowed[AL_FOURS];
+#pragma unroll
+        for (int u = 0; u < AL_FOURS; ++u) {
+            allowed[u] = next_bits[u];
+            next_bits[u] = later_bits[u];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[u][e] = next[u][e];
+        }
+#pragma unroll
+        for (int u = 0; u < AL_FOURS; ++u) {
+            load(j0 + 4 * u * AL_THREADS + AL_TURN, next_bits[u], next[u]);
+            later_bits[u] = bits_at(j0 + 4 * u * AL_THREADS + 2 * AL_TURN);
+        }
+#pragma unroll
+        for (int u = 0; u < AL_FOURS; ++u) {
+            const int j = j0 + 4 * u * AL_THREADS;
+            if (j >= high) break;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[u][e] = allowed[u] >> e & 1u ? x[u][e] : -INFINITY;
+            *reinterpret_cast<float4*>(dst + j - shift) = make_float4(x[u][0], x[u][1], x[u][2], x[u][3]);
+        }
+    }
+    // the tokens before the first four (threads 0 to 3) and behind the last (4 to 7)
+    if (tid < 8) {
+        const int j = tid < 4 ? tid : row_high + tid - 4, v = j - shift;
+        if (j >= begin && j < end && v >= 0 && (tid < 4 ? j < row_low : j >= row_low))
+            dst[v] = takes(v) ? to_float(src[v]) : -INFINITY;
+    }
+    if (p.token_offsets == nullptr && p.pending == nullptr && p.bias_offsets == nullptr) return;
+
+    // ---- the listed tokens
+    const float repeat = p.repeat ? p.repeat[row] : 1.f, presence = p.presence ? p.presence[row] : 0.f;
+    const float frequency = p.frequency ? p.frequency[row] : 0.f;
+    const int bias_first = p.bias_offsets ? p.bias_offsets[row] : 0, bias_last = p.bias_offsets ? p.bias_offsets[row + 1] : 0;
+    const unsigned to_place = (unsigned)(shift - begin), n = (unsigned)(end - begin);
+    const int* ids = p.token_ids;
+    int n_ids = 0, pending = -1;
+    if (p.dealt != nullptr) {
+        pdl_wait();                                   // the ids have been dealt out
+        const int* from = after_wait(p.dealt_from) + (size_t)row * (gridDim.x + 1) + blockIdx.x;
+        const int before = from[0];
+        n_ids = from[1] - before;
+        ids = after_wait(p.dealt) + (p.token_offsets ? p.token_offsets[row] : 0) + row + before;
+    } else {
+        if (p.token_offsets) {
+            ids += p.token_offsets[row];
+            n_ids = max(0, p.token_offsets[row + 1] - p.token_offsets[row]);
+        }
+        if (p.pending) pending = p.pending[row];
+    }
+    // places in the stretch of ids k0 + tid, + AL_THREADS, ... of a list (n or more: elsewhere)
+    auto ahead = [&](const int* list, int count, int last_id, int k0, unsigned* at) {
+        int id[AL_AHEAD];
+#pragma unroll
+        for (int e = 0; e < AL_AHEAD; ++e) {
+            const int k = k0 + e * AL_THREADS + tid;
+            id[e] = k < count ? list[k] : (k == count ? last_id : -1);
+        }
+#pragma unroll
+        for (int e = 0; e < AL_AHEAD; ++e) at[e] = id[e] >= 0 ? (unsigned)id[e] + to_place : n;
+    };
+    unsigned at[AL_AHEAD];
+    if (n_ids > 0 || pending >= 0) {
+        ahead(ids, n_ids, pending, 0, at);
+        for (int i = tid; i < (int)(n + 3) / 4; i += AL_THREADS) reinterpret_cast<int4*>(words)[i] = make_int4(0, 0, 0, 0);
+        __syncthreads();
+        for (int k0 = 0; k0 <= n_ids; k0 += AL_AHEAD * AL_THREADS) {
+            if (k0 > 0) ahead(ids, n_ids, pending, k0, at);
+#pragma unroll
+            for (int e = 0; e < AL_AHEAD; ++e)
+                if (at[e] < n) atomicAdd(&words[at[e]], 1);
+        }
+        __syncthreads();                              // the counts are whole, the scores written
+        for (int k0 = 0; k0 <= n_ids; k0 += AL_AHEAD * AL_THREADS) {
+            if (n_ids >= AL_AHEAD * AL_THREADS) ahead(ids, n_ids, pending, k0, at);
+            int c[AL_AHEAD];
+            float x[AL_AHEAD];
+#pragma unroll
+            for (int e = 0; e < AL_AHEAD; ++e) c[e] = at[e] < n ? atomicExch(&words[at[e]], 0) : 0;
+#pragma unroll
+            for (int e = 0; e < AL_AHEAD; ++e) x[e] = c[e] > 0 ? dst[(int)(at[e] - to_place)] : 0.f;
+#pragma unroll
+            for (int e = 0; e < AL_AHEAD; ++e) {
+                const int v = (int)(at[e] - to_place);
+                if (c[e] > 0 && takes(v)) {
+                    const float y = x[e] > 0.f ? x[e] / repeat : x[e] * repeat;
+                    dst[v] = y - (frequency * (float)c[e] + presence);
+                }
+            }
+        }
+    }
+    if (bias_last > bias_first) {
+        const int n_biases = bias_last - bias_first;
+        ahead(p.bias_ids + bias_first, n_biases, -1, 0, at);
+        bool here = n_biases > AL_AHEAD * AL_THREADS;
+#pragma unroll
+        for (int e = 0; e < AL_AHEAD; ++e) here = here || at[e] < n;
+        if (__syncthreads_or(here)) {
+            // three rounds over the biases of this stretch: the words' start, the largest place, the sum
+            for (int round = 0; round < 3; ++round) {
+                for (int k0 = 0; k0 < n_biases; k0 += AL_AHEAD * AL_THREADS) {
+                    if (n_biases > AL_AHEAD * AL_THREADS) ahead(p.bias_ids + bias_first, n_biases, -1, k0, at);
+#pragma unroll
+                    for (int e = 0; e < AL_AHEAD; ++e) {
+                        const int k = k0 + e * AL_THREADS + tid;
+                        if (at[e] >= n) continue;
+                        if (round == 0) words[at[e]] = -1;
+                        else if (round == 1) atomicMax(&words[at[e]], k);
+                        else if (words[at[e]] == k && takes((int)(at[e] - to_place))) dst[(int)(at[e] - to_place)] += p.bias_values[bias_first + k];
+                    }
+                }
+                __syncthreads();
+            }
+        }
+    }
+}
+
+// Scores of a block: a turn while that makes no more than some eight blocks an SM, else four turns (32 KB of counts).
+int stretch_of(int n_rows, int vocab) { return (long long)n_rows * vocab <= 8LL * 148 * AL_TURN ? AL_TURN : 4 * AL_TURN; }
+
+long long blocks_of(int n_rows, int vocab) { return ((long long)vocab + 3 + stretch_of(n_rows, vocab) - 1) / stretch_of(n_rows, vocab); }
+
+// Whether ids are dealt out first: where every block reading its row's whole list would look at more of them than at a quarter
+// of its scores.
+bool deals(long long n_ids, int n_rows, int vocab) {
+    const long long n_blocks = blocks_of(n_rows, vocab);
+    return n_blocks <= DEAL_BLOCKS && n_ids / n_rows * n_blocks > vocab / 4;
+}
+
+template <typename T>
+int launch_adjust(const AdjustParams& p, int n_rows, int n_blocks, size_t smem, cudaStream_t stream) {
+    const dim3 grid(n_blocks, n_rows);
+    const cudaError_t e = p.dealt != nullptr ? mx_launch_beside(adjust_logits_kernel<T>, grid, dim3(AL_THREADS), smem, stream, p)
+                                             : mx_launch_chained(adjust_logits_kernel<T>, grid, dim3(AL_THREADS), smem, stream, p);
     if (e != cudaSuccess) {
         mx_set_error("adjust logits: launch failed: %s", cudaGetErrorString(e));
         return (int)e;
@@ -97,20 +320,42 @@ int launch_adjust(const AdjustParams& p, int n_rows, cudaStream_t stream) {
 
 }  // namespace
 
+// Bytes of scratch of mx_adjust_logits with the same arguments: the ids by stretch, and where each stretch's begin.
+extern "C" long long mx_adjust_logits_scratch(long long n_ids, int n_rows, int vocab) {
+    if (n_rows <= 0 || vocab <= 0 || !deals(n_ids, n_rows, vocab)) return 0;
+    return 4 * (n_ids + n_rows + n_rows * (blocks_of(n_rows, vocab) + 1));
+}
+
+// n_ids: how many there are of all rows together (the size of token_ids).
 extern "C" int mx_adjust_logits(const void* logits, int dtype, long long row_stride, float* out, long long out_stride, int n_rows,
-                                int vocab, const int* token_offsets, const int* token_ids, const float* repeat,
+                                int vocab, const int* token_offsets, const int* token_ids, long long n_ids, const float* repeat,
                                 const float* presence, const float* frequency, const int* bias_offsets, const int* bias_ids,
                                 const float* bias_values, const int* mask_words, int n_masks, int mask_width,
-                                const int* mask_rows, const int* pending, cudaStream_t stream) {
+                                const int* mask_rows, const int* pending, int* scratch, cudaStream_t stream) {
     if (n_rows <= 0) return MX_OK;
     if (n_rows > 65535) MX_REFUSE("adjust logits: %d rows exceed the grid", n_rows);
-    if (vocab <= 0) MX_REFUSE("adjust logits: vocabulary of %d", vocab);
+    if (vocab <= 0 || vocab > 0x7fffffff - 65536) MX_REFUSE("adjust logits: vocabulary of %d", vocab);
     if (mask_words != nullptr && (long long)mask_width * 32 < vocab) MX_REFUSE("adjust logits: masks of %d words for %d tokens", mask_width, vocab);
     AdjustParams p;
     p.logits = logits; p.out = out; p.row_stride = row_stride; p.out_stride = out_stride; p.vocab = vocab;
     p.mask_width = mask_width; p.n_masks = mask_words ? n_masks : 0; p.token_offsets = token_offsets; p.token_ids = token_ids;
     p.bias_offsets = bias_offsets; p.bias_ids = bias_ids; p.mask_words = mask_words; p.mask_rows = mask_rows; p.pending = pending;
     p.repeat = repeat; p.presence = presence; p.frequency = frequency; p.bias_values = bias_values;
-    p.stretch = 4096;
-    return dtype == MX_DTYPE_F32 ? launch_adjust<float>(p, n_rows, stream) : launch_adjust<__nv_bfloat16>(p, n_rows, stream);
+    p.stretch = stretch_of(n_rows, vocab);
+    p.dealt = p.dealt_from = nullptr;
+    const int n_blocks = (int)blocks_of(n_rows, vocab);
+    if (deals(n_ids, n_rows, vocab)) {
+        if (scratch == nullptr) MX_REFUSE("adjust logits: long lists need scratch memory");
+        p.dealt = scratch;
+        p.dealt_from = scratch + n_ids + n_rows;
+        const cudaError_t e = mx_launch_chained(deal_ids_kernel, dim3(n_rows), dim3(DEAL_THREADS), 0, stream, p, n_blocks);
+        if (e != cudaSuccess) {
+            mx_set_error("adjust logits: launch failed: %s", cudaGetErrorString(e));
+            return (int)e;
+        }
+    }
+    const bool listed = token_offsets != nullptr || pending != nullptr || bias_offsets != nullptr;
+    const size_t smem = listed ? (size_t)p.stretch * 4 : 0;
+    return dtype == MX_DTYPE_F32 ? launch_adjust<float>(p, n_rows, n_blocks, smem, stream)
+                                 : launch_adjust<__nv_bfloat16>(p, n_rows, n_blocks, smem, stream);
 }

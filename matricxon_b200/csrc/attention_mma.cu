@@ -48,11 +48,13 @@ constexpr int MMA_WARPS = 4;        // wide tiles: 16 rows each
 constexpr int MMA_THREADS = MMA_WARPS * 32;
 constexpr int NARROW_WARPS = 8;     // narrow tiles: all warps hold the same rows and share the chunks
 constexpr int NARROW_THREADS = NARROW_WARPS * 32;
+constexpr int OWN_WARPS = 4;        // the same for OWN_KEYS
 constexpr int CHUNK = 32;
 constexpr int WIDE_STAGES = 4;      // chunks in flight per block (two pairs), wide tiles
 constexpr int NARROW_STAGES = 1;    // chunks in flight per warp, narrow tiles
 constexpr int NARROW_TABLE = 512;   // block-table entries a narrow tile's block reads ahead (8,192 positions in pages of 16)
 constexpr int SPIN_LIMIT = 1 << 22;
+constexpr int OWN_BLOCKS = 2;       // ... of which an SM holds this many
 
 struct MmaAttnParams {
     const __nv_bfloat16* q;      // [tokens][q_stride], head h at h * HD
@@ -242,13 +244,14 @@ struct One { static constexpr int value = 1; };
 struct Two { static constexpr int value = 2; };
 
 template <int HD, bool NARROW, bool BIASED, Keys KEYS>
-__global__ void __launch_bounds__(NARROW ? NARROW_THREADS : MMA_THREADS, NARROW ? 1 : 3)
+__global__ void __launch_bounds__(NARROW && KEYS == ALL_KEYS ? NARROW_THREADS : MMA_THREADS, NARROW ? (KEYS == ALL_KEYS ? 1 : OWN_BLOCKS) : 3)
 attention_mma_kernel(const MmaAttnParams p) {
+    constexpr int N_WARPS = NARROW && KEYS == ALL_KEYS ? NARROW_WARPS : OWN_WARPS;   // of a narrow tile
     constexpr int KB = HD / 32;                 // 32-wide blocks of the head dim
     constexpr int NB = HD / 8;                  // 8-wide output column blocks
     constexpr int STAGE_ELEMS = 2 * CHUNK * HD; // keys then values
     constexpr int TILE_ROWS = NARROW ? 16 : 16 * MMA_WARPS;
-    constexpr int N_STAGES = NARROW ? NARROW_STAGES * NARROW_WARPS : WIDE_STAGES;
+    constexpr int N_STAGES = NARROW ? NARROW_STAGES * N_WARPS : WIDE_STAGES;
     extern __shared__ __align__(128) unsigned char smem_raw[];
     __nv_bfloat16* stages = reinterpret_cast<__nv_bfloat16*>(smem_raw);
     __shared__ __align__(8) unsigned long long bars[N_STAGES];
@@ -381,12 +384,12 @@ attention_mma_kernel(const MmaAttnParams p) {
     __nv_bfloat16* my_stages = stages + (size_t)(NARROW ? warp : 0) * NARROW_STAGES * STAGE_ELEMS;
     unsigned long long* my_bars = bars + (NARROW ? warp : 0) * NARROW_STAGES;
     const int my_first = c_begin + warp;
-    const int my_count = NARROW && my_first < c_end ? (c_end - my_first + NARROW_WARPS - 1) / NARROW_WARPS : 0;
+    const int my_count = NARROW && my_first < c_end ? (c_end - my_first + N_WARPS - 1) / N_WARPS : 0;
     // This warp's chunks find their pages in the row read ahead at the top (entries beyond what was
     // kept are looked up in global memory).
     auto cached_for = [&](int i) -> const int* {
         const int pages = CHUNK >> p.page_shift;
-        const int first = chunk_of(my_first + NARROW_WARPS * i) * pages;
+        const int first = chunk_of(my_first + N_WARPS * i) * pages;
         return first + pages <= min(p.bt_stride, NARROW_TABLE) ? narrow_table + first : nullptr;
     };
     const bool first_is_old = (chunk_of(my_first) + 1) * CHUNK <= ctx;
@@ -628,28 +631,28 @@ attention_mma_kernel(const MmaAttnParams p) {
             if (NARROW_STAGES > 1 && i + 1 < my_count) {
                 const int nx = (i + 1) % NARROW_STAGES;
                 __nv_bfloat16* ks = my_stages + (size_t)nx * STAGE_ELEMS;
-                issue_chunk_warp<HD>(p, ks, ks + CHUNK * HD, &my_bars[nx], chunk_of(my_first + NARROW_WARPS * (i + 1)) * CHUNK,
+                issue_chunk_warp<HD>(p, ks, ks + CHUNK * HD, &my_bars[nx], chunk_of(my_first + N_WARPS * (i + 1)) * CHUNK,
                                      lo_tile, hi_tile, kept, bt, kbase, vbase, page_stride, lane, cached_for(i + 1));
             }
             __syncwarp();
             mbar_wait(&my_bars[st], (unsigned)((i / NARROW_STAGES) & 1), p.status);
             const __nv_bfloat16* ks = my_stages + (size_t)st * STAGE_ELEMS;
             {
-                const int c0 = chunk_of(my_first + NARROW_WARPS * i) * CHUNK;
+                const int c0 = chunk_of(my_first + N_WARPS * i) * CHUNK;
                 compute(One{}, ks, ks + CHUNK * HD, ks, ks + CHUNK * HD, c0, c0);
             }
             __syncwarp();                         // the stage may be refilled from here on
             if (NARROW_STAGES == 1 && i + 1 < my_count)
                 issue_chunk_warp<HD>(p, my_stages, my_stages + CHUNK * HD, &my_bars[0],
-                                     chunk_of(my_first + NARROW_WARPS * (i + 1)) * CHUNK, lo_tile, hi_tile, kept, bt, kbase,
+                                     chunk_of(my_first + N_WARPS * (i + 1)) * CHUNK, lo_tile, hi_tile, kept, bt, kbase,
                                      vbase, page_stride, lane, cached_for(i + 1));
         }
         // ---- combine the warps' partial results through shared memory (stages are free)
         __syncthreads();
         constexpr int RS = HD + 8;                                      // row stride: the warps' stores hit every bank once
         float* red_o = reinterpret_cast<float*>(smem_raw);              // [warp][16][RS]
-        float* red_ml = red_o + NARROW_WARPS * 16 * RS;                 // [warp][16][2]
-        __shared__ float weight_of[NARROW_WARPS][16], sum_of[16], max_of[16];
+        float* red_ml = red_o + N_WARPS * 16 * RS;                 // [warp][16][2]
+        __shared__ float weight_of[N_WARPS][16], sum_of[16], max_of[16];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = g + 8 * i;
@@ -664,11 +667,11 @@ attention_mma_kernel(const MmaAttnParams p) {
         }
         __syncthreads();
         // each warp's weight for each row, once (one thread per pair), and each row's maximum and sum
-        if (tid < NARROW_WARPS * 16) {
+        if (tid < N_WARPS * 16) {
             const int r = tid & 15, w = tid >> 4;
             float m = -INFINITY;
 #pragma unroll
-            for (int w2 = 0; w2 < NARROW_WARPS; ++w2) m = fmaxf(m, red_ml[((size_t)w2 * 16 + r) * 2]);
+            for (int w2 = 0; w2 < N_WARPS; ++w2) m = fmaxf(m, red_ml[((size_t)w2 * 16 + r) * 2]);
             const float mw = red_ml[((size_t)w * 16 + r) * 2];
             weight_of[w][r] = (mw == -INFINITY) ? 0.f : fast_exp2(mw - m);
             if (w == 0) max_of[r] = m;
@@ -677,18 +680,18 @@ attention_mma_kernel(const MmaAttnParams p) {
         if (tid < 16) {
             float l = 0.f;
 #pragma unroll
-            for (int w = 0; w < NARROW_WARPS; ++w) l += red_ml[((size_t)w * 16 + tid) * 2 + 1] * weight_of[w][tid];
+            for (int w = 0; w < N_WARPS; ++w) l += red_ml[((size_t)w * 16 + tid) * 2 + 1] * weight_of[w][tid];
             sum_of[tid] = l;
         }
         const bool whole = KEYS == ALL_KEYS && p.n_splits == 1;
         if (whole) __syncthreads();                // the only reader of sum_of among other threads
         const int rows_here = min(16, n_rows - tile_row0);
         const float ln2 = 0.6931471805599453f;
-        for (int idx = tid; idx < rows_here * (HD / 4); idx += NARROW_THREADS) {
+        for (int idx = tid; idx < rows_here * (HD / 4); idx += 32 * N_WARPS) {
             const int r = idx / (HD / 4), d = 4 * (idx - r * (HD / 4));
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < NARROW_WARPS; ++w) {
+            for (int w = 0; w < N_WARPS; ++w) {
                 const float4 v = *reinterpret_cast<const float4*>(red_o + ((size_t)w * 16 + r) * RS + d);
                 const float wgt = weight_of[w][r];
                 acc.x += v.x * wgt; acc.y += v.y * wgt; acc.z += v.z * wgt; acc.w += v.w * wgt;
@@ -788,9 +791,11 @@ attention_mma_kernel(const MmaAttnParams p) {
 template <int HD, bool NARROW, bool BIASED, Keys KEYS>
 int launch_mma_kernel(const MmaAttnParams& p, cudaStream_t stream) {
     const size_t stage_bytes = 2 * (size_t)CHUNK * HD * sizeof(__nv_bfloat16);
-    size_t smem = stage_bytes * (NARROW ? NARROW_STAGES * NARROW_WARPS : WIDE_STAGES);
+    constexpr int n_warps = NARROW && KEYS == ALL_KEYS ? NARROW_WARPS : OWN_WARPS;
+    const dim3 block(NARROW ? 32 * n_warps : MMA_THREADS);
+    size_t smem = stage_bytes * (NARROW ? NARROW_STAGES * n_warps : WIDE_STAGES);
     if (NARROW) {
-        const size_t reduce = (size_t)NARROW_WARPS * 16 * (HD + 8 + 2) * sizeof(float);
+        const size_t reduce = (size_t)n_warps * 16 * (HD + 8 + 2) * sizeof(float);
         if (reduce > smem) smem = reduce;
     }
     if (smem + 1024 > 48 * 1024) {   // the kernel also has a little static shared memory
@@ -800,15 +805,14 @@ int launch_mma_kernel(const MmaAttnParams& p, cudaStream_t stream) {
     }
     dim3 grid(p.n_tiles, p.n_kv_heads, p.n_splits);
     if (KEYS == OWN_KEYS && p.shared.beside) {
-        const cudaError_t e = mx_launch_beside(attention_mma_kernel<HD, NARROW, BIASED, KEYS>, grid,
-                                               dim3(NARROW ? NARROW_THREADS : MMA_THREADS), smem, stream, p);
+        const cudaError_t e = mx_launch_beside(attention_mma_kernel<HD, NARROW, BIASED, KEYS>, grid, block, smem, stream, p);
         if (e != cudaSuccess) {
             mx_set_error("attention: launch failed: %s", cudaGetErrorString(e));
             return (int)e;
         }
         return MX_OK;
     }
-    mx_launch_chained(attention_mma_kernel<HD, NARROW, BIASED, KEYS>, grid, dim3(NARROW ? NARROW_THREADS : MMA_THREADS), smem, stream, p);
+    mx_launch_chained(attention_mma_kernel<HD, NARROW, BIASED, KEYS>, grid, block, smem, stream, p);
     return mx_launch_status();
 }
 

@@ -60,26 +60,37 @@ __device__ __forceinline__ void unpack16<__nv_bfloat16>(const uint4& raw, float*
     }
 }
 
+// Sixteen bytes on their way to shared memory; zeros where `there` is false (nothing is read then).
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src),
+                 "r"(there ? 16 : 0)
+                 : "memory");
+}
+
 // SHARED: a tile is sixteen (token, head) rows of a group, token-major. Otherwise up to sixteen heads of one token.
+// Two stages: a chunk's keys [key][dim] and values [dim][key], as they lie in the pages, are on their way while the chunk
+// before is computed on. Both are kept with their 16-byte pieces swizzled, so that 32 lanes on 32 keys (scores) and on 32
+// dimensions (values) meet no bank twice.
 template <typename T, int SLOTS, bool SHARED>
 __global__ void __launch_bounds__(SH_THREADS)
 shared_simt_kernel(const SharedAttnParams p) {
     constexpr int E = Vec16<T>::E;
+    constexpr int RUNS = SH_KEYS / E;                         // 16-byte pieces of a dimension's values
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ int row_token[SH_ROWS], row_head[SH_ROWS], row_lo[SH_ROWS], row_hi[SH_ROWS];
     __shared__ float row_alpha[SH_ROWS], row_m[SH_ROWS], row_l[SH_ROWS];
-    const int hd = p.head_dim, cpr = hd / E;                  // 16-byte pieces a key
-    const int swz_mask = (cpr % 8 == 0) ? 7 : 0;
+    const int hd = p.head_dim, cpr = hd / E;                  // 16-byte pieces of a key
+    const int swz_mask = (cpr % 8 == 0) ? 7 : (cpr % 4 == 0 ? 3 : (cpr % 2 == 0 ? 1 : 0));
     float* q_s = reinterpret_cast<float*>(smem_raw);          // [SH_ROWS][hd]
     float* p_s = q_s + SH_ROWS * hd;                          // [SH_ROWS][SH_KEYS]
-    uint4* k_s = reinterpret_cast<uint4*>(p_s + SH_ROWS * SH_KEYS);   // [SH_KEYS][cpr], swizzled
-    uint4* v_s = k_s + SH_KEYS * cpr;                         // [SH_KEYS][cpr]
+    uint4* stages = reinterpret_cast<uint4*>(p_s + SH_ROWS * SH_KEYS);
+    const int stage_pieces = SH_KEYS * cpr + hd * RUNS;       // keys, then values
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int kh = blockIdx.y, split = blockIdx.z;
 
-    pdl_wait();
+    if (SHARED || !p.shared.beside) pdl_wait();
     pdl_trigger();
-    int seq, rows, first_token, first_row;
+    int seq = 0, rows = 0, first_token = 0, first_row = 0;
     if (SHARED) {
         const GroupTile found = find_group_tile(p.shared, p.cu_q, blockIdx.x, SH_ROWS, p.group, lane);
         if (found.tokens <= 0) return;
@@ -90,9 +101,11 @@ shared_simt_kernel(const SharedAttnParams p) {
         first_token = blockIdx.x / parts;
         first_row = (blockIdx.x - first_token * parts) * SH_ROWS;
         rows = min(SH_ROWS, p.group - first_row);
-        if (first_token >= p.cu_q[p.shared.n_seqs]) return;
-        seq = p.shared.tok_seq[first_token];
-        if (seq < 0 || seq >= p.shared.n_seqs) return;
+        seq = first_token < p.cu_q[p.shared.n_seqs] ? p.shared.tok_seq[first_token] : -1;
+        if (seq < 0 || seq >= p.shared.n_seqs) {
+            pdl_wait();
+            return;
+        }
     }
     if (tid < rows) {
         const int r = first_row + tid, t = r / p.group;
@@ -116,10 +129,43 @@ shared_simt_kernel(const SharedAttnParams p) {
     const int per_split = (n_chunks + p.n_splits - 1) / p.n_splits;
     const int c_begin = split * per_split, c_end = min(n_chunks, c_begin + per_split);
 
-    for (int i = tid; i < rows * hd; i += SH_THREADS) {
-        const int r = i / hd, d = i - r * hd;
-        q_s[i] = to_float(reinterpret_cast<const T*>(p.q)[(size_t)row_token[r] * p.q_stride + (size_t)row_head[r] * hd + d]);
-    }
+    const int* bt = p.block_tables + (size_t)seq * p.bt_stride;
+    const T* cache = reinterpret_cast<const T*>(p.cache);
+    const size_t head_stride = (size_t)p.page_size * hd;
+    auto page_of = [&](int key) -> long long {
+        const int lp = key / p.page_size;
+        const long long page = lp < p.bt_stride ? bt[lp] : -1;
+        return page >= 0 && page < p.n_pages ? page : -1;
+    };
+    auto bring = [&](int c) {
+        uint4* k_s = stages + (size_t)(c & 1) * stage_pieces;
+        uint4* v_s = k_s + SH_KEYS * cpr;
+        const int c0 = (first_chunk + c) * SH_KEYS;
+        // a warp a key
+#pragma unroll 4
+        for (int j = warp; j < SH_KEYS; j += SH_WARPS) {
+            const int key = c0 + j;
+            const bool seen = key >= lo && key <= hi;
+            const long long page = seen ? page_of(key) : -1;
+            if (seen && page < 0 && lane == 0) atomicOr(p.status, MX_STATUS_BAD_PAGE);
+            const T* from = cache + ((size_t)max(page, 0LL) * 2 * p.n_kv_heads + kh) * head_stride + (size_t)(key % p.page_size) * hd;
+            for (int piece = lane; piece < cpr; piece += 32)
+                copy16(&k_s[j * cpr + (piece ^ (j & swz_mask))], page >= 0 ? from + (size_t)piece * E : cache, page >= 0);
+        }
+        // a run of E keys lies inside a page: a thread keeps to one run and walks the dimensions
+        const int run = tid % RUNS, key0 = c0 + run * E;
+        const long long page = key0 <= hi && key0 + E - 1 >= lo ? page_of(key0) : -1;
+        const T* from = cache + ((size_t)max(page, 0LL) * 2 * p.n_kv_heads + p.n_kv_heads + kh) * head_stride + key0 % p.page_size;
+#pragma unroll 4
+        for (int d = tid / RUNS; d < hd; d += SH_THREADS / RUNS)
+            copy16(&v_s[d * RUNS + (run ^ (d & (RUNS - 1)))], page >= 0 ? from + (size_t)d * p.page_size : cache, page >= 0);
+    };
+    if (c_begin < c_end) bring(c_begin);
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+
+    for (int r = warp; r < rows; r += SH_WARPS)
+        for (int d = lane; d < hd; d += 32)
+            q_s[r * hd + d] = to_float(reinterpret_cast<const T*>(p.q)[(size_t)row_token[r] * p.q_stride + (size_t)row_head[r] * hd + d]);
     float acc[SH_ROWS][SLOTS];
 #pragma unroll
     for (int r = 0; r < SH_ROWS; ++r)
@@ -129,47 +175,12 @@ shared_simt_kernel(const SharedAttnParams p) {
 #pragma unroll
     for (int i = 0; i < SH_ROWS_PER_WARP; ++i) { m_run[i] = -INFINITY; l_run[i] = 0.f; }
 
-    const int* bt = p.block_tables + (size_t)seq * p.bt_stride;
-    const T* cache = reinterpret_cast<const T*>(p.cache);
-    const size_t head_stride = (size_t)p.page_size * hd;
     for (int c = c_begin; c < c_end; ++c) {
         const int c0 = (first_chunk + c) * SH_KEYS;
-        // ---- keys (zeros for those that no row sees)
-        for (int item = tid; item < SH_KEYS * cpr; item += SH_THREADS) {
-            const int j = item / cpr, piece = item - j * cpr, key = c0 + j;
-            uint4 raw = make_uint4(0, 0, 0, 0);
-            if (key >= lo && key <= hi) {
-                const int lp = key / p.page_size;
-                const long long page = lp < p.bt_stride ? bt[lp] : -1;
-                if (page < 0 || page >= p.n_pages) {
-                    if (piece == 0) atomicOr(p.status, MX_STATUS_BAD_PAGE);
-                } else {
-                    raw = *reinterpret_cast<const uint4*>(cache + ((size_t)page * 2 * p.n_kv_heads + kh) * head_stride +
-                                                          (size_t)(key - lp * p.page_size) * hd + (size_t)piece * E);
-                }
-            }
-            k_s[j * cpr + (piece ^ (j & swz_mask))] = raw;
-        }
-        // ---- values: memory has [dim][slot], shared memory wants [key][dim]; runs of E keys lie inside a page
-        {
-            constexpr int RUNS = SH_KEYS / E;
-            T* v_t = reinterpret_cast<T*>(v_s);
-            for (int item = tid; item < hd * RUNS; item += SH_THREADS) {
-                const int d = item / RUNS, run = item - d * RUNS, key0 = c0 + run * E;
-                uint4 raw = make_uint4(0, 0, 0, 0);
-                if (key0 <= hi && key0 + E - 1 >= lo) {
-                    const int lp = key0 / p.page_size;
-                    const long long page = lp < p.bt_stride ? bt[lp] : -1;
-                    if (page >= 0 && page < p.n_pages)
-                        raw = *reinterpret_cast<const uint4*>(cache + ((size_t)page * 2 * p.n_kv_heads + p.n_kv_heads + kh) * head_stride +
-                                                              (size_t)d * p.page_size + (key0 - lp * p.page_size));
-                }
-                const T* elems = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    v_t[(size_t)(run * E + e) * hd + d] = key0 + e >= lo && key0 + e <= hi ? elems[e] : from_float<T>(0.f);
-            }
-        }
+        const uint4* k_s = stages + (size_t)(c & 1) * stage_pieces;
+        uint4* v_s = const_cast<uint4*>(k_s) + SH_KEYS * cpr;
+        if (c + 1 < c_end) bring(c + 1);
+        asm volatile("cp.async.commit_group;\ncp.async.wait_group 1;\n" ::: "memory");
         __syncthreads();
         // ---- scores: a lane a key, this warp's rows are warp, warp + 4, ...
         float s[SH_ROWS_PER_WARP];
@@ -212,6 +223,15 @@ shared_simt_kernel(const SharedAttnParams p) {
                 if (lane == 0) row_alpha[r] = alpha;
             }
         }
+        if (c0 < lo || c0 + SH_KEYS - 1 > hi) {
+            // slots that no row sees may hold anything (0 times NaN)
+            T* v_t = reinterpret_cast<T*>(v_s);
+            for (int d = warp; d < hd; d += SH_WARPS) {
+                const int run = lane / E;
+                if (c0 + lane < lo || c0 + lane > hi)
+                    v_t[(size_t)(d * RUNS + (run ^ (d & (RUNS - 1)))) * E + lane % E] = from_float<T>(0.f);
+            }
+        }
         __syncthreads();
         // ---- weighted values: a thread a dimension (or two), all rows
 #pragma unroll
@@ -221,15 +241,20 @@ shared_simt_kernel(const SharedAttnParams p) {
 #pragma unroll
                 for (int r = 0; r < SH_ROWS; ++r)
                     if (r < rows) acc[r][slot] *= row_alpha[r];
-                const T* vcol = reinterpret_cast<const T*>(v_s) + d;
-                for (int j = 0; j < SH_KEYS; j += 4) {
-                    const float v0 = to_float(vcol[(size_t)(j + 0) * hd]), v1 = to_float(vcol[(size_t)(j + 1) * hd]);
-                    const float v2 = to_float(vcol[(size_t)(j + 2) * hd]), v3 = to_float(vcol[(size_t)(j + 3) * hd]);
+#pragma unroll 2
+                for (int run = 0; run < RUNS; ++run) {
+                    float v[E];
+                    unpack16<T>(v_s[d * RUNS + (run ^ (d & (RUNS - 1)))], v);
 #pragma unroll
                     for (int r = 0; r < SH_ROWS; ++r)
                         if (r < rows) {
-                            const float4 pp = *reinterpret_cast<const float4*>(p_s + r * SH_KEYS + j);
-                            acc[r][slot] = fmaf(pp.w, v3, fmaf(pp.z, v2, fmaf(pp.y, v1, fmaf(pp.x, v0, acc[r][slot]))));
+                            const float4* pp = reinterpret_cast<const float4*>(p_s + r * SH_KEYS + run * E);
+#pragma unroll
+                            for (int e4 = 0; e4 < E / 4; ++e4) {
+                                const float4 w = pp[e4];
+                                acc[r][slot] = fmaf(w.w, v[4 * e4 + 3], fmaf(w.z, v[4 * e4 + 2],
+                                               fmaf(w.y, v[4 * e4 + 1], fmaf(w.x, v[4 * e4], acc[r][slot]))));
+                            }
                         }
                 }
             }
@@ -253,6 +278,7 @@ shared_simt_kernel(const SharedAttnParams p) {
             }
             if (tid == 0) { p.part_ml[base * 2] = row_m[r]; p.part_ml[base * 2 + 1] = row_l[r]; }
         }
+    if (!SHARED) pdl_wait();                 // whoever waits for this kernel waits for the shared keys' too
 }
 
 // The join: a warp a (token, head), four dimensions a lane. A token of no sequence is left alone.
@@ -310,12 +336,14 @@ shared_join_kernel(const float* part_o, const float* part_ml, T* out, int out_st
 
 template <typename T, int SLOTS, bool SHARED>
 int launch_simt(const SharedAttnParams& p, unsigned n_tiles, cudaStream_t stream) {
-    const size_t smem = (size_t)SH_ROWS * p.head_dim * 4 + SH_ROWS * SH_KEYS * 4 + 2 * (size_t)SH_KEYS * p.head_dim * sizeof(T);
+    const size_t smem = (size_t)SH_ROWS * p.head_dim * 4 + SH_ROWS * SH_KEYS * 4 + 4 * (size_t)SH_KEYS * p.head_dim * sizeof(T);
     if (smem > 47 * 1024 && cudaFuncSetAttribute(shared_simt_kernel<T, SLOTS, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  (int)smem) != cudaSuccess)
         MX_REFUSE("attention over shared keys: cannot reserve %zu bytes of shared memory", smem);
-    const cudaError_t e = mx_launch_chained(shared_simt_kernel<T, SLOTS, SHARED>, dim3(n_tiles, p.n_kv_heads, p.n_splits),
-                                            dim3(SH_THREADS), smem, stream, p);
+    const dim3 grid(n_tiles, p.n_kv_heads, p.n_splits);
+    const cudaError_t e = !SHARED && p.shared.beside
+                              ? mx_launch_beside(shared_simt_kernel<T, SLOTS, SHARED>, grid, dim3(SH_THREADS), smem, stream, p)
+                              : mx_launch_chained(shared_simt_kernel<T, SLOTS, SHARED>, grid, dim3(SH_THREADS), smem, stream, p);
     if (e != cudaSuccess) {
         mx_set_error("attention over shared keys: launch failed: %s", cudaGetErrorString(e));
         return (int)e;
@@ -356,11 +384,14 @@ SharedPlan make_plan(int dtype, int head_dim, int page_size, bool aligned, int n
     const int shared_rows = tc ? 128 / group * group : (mma ? 64 : SH_ROWS);
     plan.shared_tiles = (int)min(rows / shared_rows + n_groups, rows);
     plan.own_tiles = mma ? (plan.narrow ? n_seqs : (int)min(rows / 64 + n_seqs, rows)) : n_tokens * ((group + SH_ROWS - 1) / SH_ROWS);
-    const int shared_keys = tc ? 128 : 32;
-    const int shared_chunks = (max(max_shared_len, 1) + shared_keys - 1) / shared_keys, own_chunks = max(max_own_len, 1) / 32 + 1;
-    const int shared_blocks = plan.shared_tiles * n_kv_heads, own_blocks = plan.own_tiles * n_kv_heads;
-    plan.shared_parts = max_shared_len <= 0 ? 0 : max(1, min(min((tc ? n_sm : 4 * n_sm) / max(shared_blocks, 1), shared_chunks / (tc ? 2 : 4)), 32));
-    plan.own_parts = max(1, min(min((plan.narrow ? n_sm : 4 * n_sm) / max(own_blocks, 1), own_chunks / 8), 32));
+    // A share of the shared keys a block is worth it from two chunks on (128 keys with tcgen05, a block an SM; else 32, four an
+    // SM); the own keys' from four chunks a block (its four warps take one each; wide tiles two pairs), or two. With few tiles
+    // the parts fill the GPU; with many they only even out.
+    const int shared_chunks = (max(max_shared_len, 1) + (tc ? 127 : 31)) / (tc ? 128 : 32), own_chunks = max(max_own_len, 1) / 32 + 1;
+    const long long shared_blocks = (rows + shared_rows - 1) / shared_rows * n_kv_heads, own_blocks = (long long)plan.own_tiles * n_kv_heads;
+    const long long room = tc ? n_sm : 4 * n_sm, own_room = plan.narrow ? 2 * n_sm : 4 * n_sm;
+    plan.shared_parts = max_shared_len <= 0 ? 0 : (int)max(1LL, min(min(room / max(shared_blocks, 1LL), (long long)shared_chunks / 2), 32LL));
+    plan.own_parts = (int)max(1LL, min(min(own_room / max(own_blocks, 1LL), (long long)own_chunks / (plan.narrow ? 4 : 2)), 32LL));
     return plan;
 }
 
@@ -448,7 +479,7 @@ extern "C" int mx_paged_attention_shared(const void* q, int dtype, int q_stride,
                                            : launch_simt<__nv_bfloat16, 1, true>(p, plan.shared_tiles, stream);
         }
         if (rc != MX_OK) return rc;
-        p.shared.beside = plan.path > 0;
+        p.shared.beside = 1;
     }
     if (plan.path > 0) {
         rc = mx_attention_mma_shared(q, q_stride, cache, n_pages, page_size, block_tables, bt_stride, cu_q, context_lens, n_heads,

@@ -15,7 +15,7 @@
 // changed (lengths, free pages), so a step can be laid out twice.
 //
 // Every block adds up all sequences' lengths for itself (a sequence a thread, 8 to 20 bytes each out of L2), which spares a
-// second launch or a wait between blocks, and then lays out its few sequences. A step that does not fit (more rows than the
+// second launch or a wait between blocks; it then lays out its few sequences. A step that does not fit (more rows than the
 // buffers hold, more pages than there are, a length out of range) sets MX_STATUS_BAD_STEP and every block leaves an empty step:
 // all -1, nothing taken, `tables` as they were.
 // The launch after this one must not begin early: attention kernels read tables and lengths before they wait for what ran
@@ -24,9 +24,9 @@
 
 namespace {
 
-constexpr int ST_THREADS = 256;
+constexpr int ST_THREADS = 512;
 constexpr int ST_OWN = 64;              // sequences a block lays out, at most
-constexpr int ST_SLICE = 4096;          // block-table entries of a sequence that one block writes
+constexpr int ST_SLICE = 16384;         // block-table entries of a sequence that one block writes
 
 struct StepTablesParams {
     const int *q_lens, *context_lens, *rows, *shared_rows, *shared_pages, *free_pages, *n_free;
@@ -48,7 +48,7 @@ __device__ __forceinline__ Sequence read_sequence(const StepTablesParams& p, int
     v.row = p.rows ? p.rows[s] : s;
     v.shared_row = p.shared_rows ? p.shared_rows[s] : -1;
     v.shared = v.shared_row >= 0 ? p.shared_pages[s] : 0;
-    const long long most = (long long)p.width * p.page_size;
+    const long long most = min((long long)p.width * p.page_size, 0x7fffffffLL);
     v.fits = v.q >= 0 && v.context >= 0 && v.row >= -1 && v.row < p.n_rows && v.shared_row < p.n_rows &&
              (long long)v.context + v.q <= most && (v.row >= 0 || v.q == 0) && v.shared >= 0 &&
              (long long)v.shared * p.page_size <= v.context;
@@ -56,58 +56,55 @@ __device__ __forceinline__ Sequence read_sequence(const StepTablesParams& p, int
         v.q = v.context = v.shared = 0;
         v.row = v.shared_row = -1;
     }
-    v.have = (int)(((long long)v.context + p.page_size - 1) / p.page_size);
-    v.need = (int)(((long long)v.context + v.q + p.page_size - 1) / p.page_size) - v.have;
+    // (sums of two numbers below 2^31 and a page fit 32 bits without a sign)
+    v.have = (int)(((unsigned)v.context + (unsigned)p.page_size - 1u) / (unsigned)p.page_size);
+    v.need = (int)(((unsigned)v.context + (unsigned)v.q + (unsigned)p.page_size - 1u) / (unsigned)p.page_size) - v.have;
     return v;
 }
 
 __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTablesParams p) {
-    __shared__ long long warp_q[ST_THREADS / 32], warp_need[ST_THREADS / 32];
-    __shared__ long long own_q[ST_OWN], own_need[ST_OWN];
+    __shared__ long long warp_total[ST_THREADS / 32];
+    __shared__ int warp_sums[3][ST_THREADS / 32];
     __shared__ Sequence own[ST_OWN];
     __shared__ int repeated[ST_OWN];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int first = blockIdx.x * p.per_block, last = min(p.n_seqs, first + p.per_block);
     pdl_wait();
-    for (int i = tid; i < ST_OWN; i += ST_THREADS) repeated[i] = 0;
 
-    // ---- running sums over all sequences, a sequence a thread
-    long long q_before = 0, need_before = 0;
+    // ---- what all sequences bring and take, and what those before this block's do
+    long long q_all = 0;
+    int q_before = 0, need_before = 0, need_all = 0;         // (before: wrong only where the step does not fit anyway)
     bool fits = true;
-    for (int s0 = 0; s0 < p.n_seqs; s0 += ST_THREADS) {
-        const int s = s0 + tid;
-        Sequence v = {};
-        v.row = -1;
-        v.fits = true;
-        if (s < p.n_seqs) v = read_sequence(p, s);
+#pragma unroll 2
+    for (int s = tid; s < p.n_seqs; s += ST_THREADS) {
+        const Sequence v = read_sequence(p, s);
         fits = fits && v.fits;
-        long long q = v.q, need = v.need;
+        q_all += v.q;
+        need_all += v.need;
+        if (s < first) { q_before += v.q; need_before += v.need; }
+        else if (s < last) own[s - first] = v;
+    }
+    for (int i = tid; i < ST_OWN; i += ST_THREADS) repeated[i] = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long a = __shfl_up_sync(0xffffffffu, q, o), b = __shfl_up_sync(0xffffffffu, need, o);
-            if (lane >= o) { q += a; need += b; }
-        }
-        if (lane == 31) { warp_q[warp] = q; warp_need[warp] = need; }
-        __syncthreads();
-        long long q_all = 0, need_all = 0;
+    for (int o = 16; o > 0; o >>= 1) q_all += __shfl_xor_sync(0xffffffffu, q_all, o);
+    q_before = (int)__reduce_add_sync(0xffffffffu, (unsigned)q_before);
+    need_before = (int)__reduce_add_sync(0xffffffffu, (unsigned)need_before);
+    need_all = (int)__reduce_add_sync(0xffffffffu, (unsigned)need_all);
+    if (lane == 0) {
+        warp_total[warp] = q_all;
+        warp_sums[0][warp] = q_before; warp_sums[1][warp] = need_before; warp_sums[2][warp] = need_all;
+    }
+    const bool all_fit = __syncthreads_and(fits);
+    q_all = 0;
+    q_before = need_before = need_all = 0;
 #pragma unroll
-        for (int w = 0; w < ST_THREADS / 32; ++w) {
-            if (w == warp) { q += q_all; need += need_all; }
-            q_all += warp_q[w];
-            need_all += warp_need[w];
-        }
-        if (s >= first && s < last) {
-            own[s - first] = v;
-            own_q[s - first] = q_before + q - v.q;
-            own_need[s - first] = need_before + need - v.need;
-        }
-        q_before += q_all;
-        need_before += need_all;
-        __syncthreads();
+    for (int w = 0; w < ST_THREADS / 32; ++w) {
+        q_all += warp_total[w];
+        q_before += warp_sums[0][w]; need_before += warp_sums[1][w]; need_all += warp_sums[2][w];
     }
     const int n_free = min(*p.n_free, p.n_free_most);
-    const bool possible = __syncthreads_and(fits) && q_before <= p.n_tokens && need_before <= n_free;
-    const int total = possible ? (int)q_before : 0;
+    const bool possible = all_fit && q_all <= p.n_tokens && need_all <= n_free;
+    const int total = possible ? (int)q_all : 0;
     // a row that an earlier sequence has already: the later one is laid out as empty
     if (possible && p.rows) {
         for (int s = tid; s < last; s += ST_THREADS) {
@@ -120,15 +117,18 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTable
     }
     if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) {
         p.cu_q[0] = 0;
-        *p.taken = possible ? (int)need_before : 0;
+        *p.taken = possible ? need_all : 0;
         if (!possible) atomicOr(p.status, MX_STATUS_BAD_STEP);
     }
 
     // ---- this block's sequences
     const int k_begin = blockIdx.y * ST_SLICE, k_end = min(p.width, k_begin + ST_SLICE);
+    int begin_next = q_before, taken_next = need_before;
     for (int s = first; s < last; ++s) {
         const Sequence v = own[s - first];
-        const int begin = (int)own_q[s - first], taken = (int)own_need[s - first];
+        const int begin = begin_next, taken = taken_next;
+        begin_next += v.q;
+        taken_next += v.need;
         const bool there = possible && v.row >= 0 && !repeated[s - first];
         if (blockIdx.y == 0 && tid == 0) {
             p.cu_q[s + 1] = possible ? begin + v.q : 0;
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTable
         const int seen_from = first_visible_key(v.context, p.window) / p.page_size;
         int* out = p.block_tables + (size_t)s * p.width;
         bool bad_page = false;
-#pragma unroll 4
+#pragma unroll 8
         for (int k = k_begin + tid; k < k_end; k += ST_THREADS) {
             int page = -1;
             if (k < end) {
@@ -193,6 +193,7 @@ extern "C" int mx_step_tables(const int* q_lens, const int* context_lens, const 
     if (n_seqs <= 0) MX_REFUSE("step tables: a step of %d sequences", n_seqs);
     if (width <= 0 || n_rows <= 0 || n_tokens < 0) MX_REFUSE("step tables: %d rows of %d entries, %d tokens", n_rows, width, n_tokens);
     if (page_size <= 0) MX_REFUSE("step tables: pages of %d positions", page_size);
+    if ((long long)n_seqs * width > 0x7fffffffLL) MX_REFUSE("step tables: %d tables of %d entries", n_seqs, width);
     if (n_pages <= 0 || n_pages * page_size > 0x7fffffffLL) MX_REFUSE("step tables: %lld pages of %d positions have no 32-bit slots", n_pages, page_size);
     if (keep_first < 0) MX_REFUSE("step tables: %d kept positions", keep_first);
     if ((shared_rows == nullptr) != (shared_pages == nullptr)) MX_REFUSE("step tables: shared rows and shared pages go together");

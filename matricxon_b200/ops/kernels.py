@@ -668,25 +668,30 @@ def mma_attention_supported(dtype: torch.dtype, head_dim: int, page_size: int, q
             and q_stride % 8 == 0)
 
 
-def _need_here(*tensors: tuple[str, torch.Tensor | None]) -> None:
-    """Launches go to the current device's current stream: tensors of another device are refused."""
-    here = torch.cuda.current_device() if torch.cuda.is_available() else None
-    for name, tensor in tensors:
+def _here(name: str, tensor: torch.Tensor) -> int:
+    """The device that launches go to, which has to be ``tensor``'s: the current one, one per process."""
+    if not tensor.is_cuda:
+        raise KernelLibraryError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    here = torch.cuda.current_device()
+    if _device_index is not None and here != _device_index:
+        raise KernelLibraryError(f"kernels of this process run on cuda:{_device_index}, the current device is cuda:{here}")
+    if tensor.get_device() != here:
+        raise KernelLibraryError(f"{name} is on {tensor.device}, kernels run on cuda:{here}")
+    return here
+
+
+def _need_all(here: int, dtype: torch.dtype, *wanted: tuple[str, torch.Tensor | None, tuple | None]) -> None:
+    """Every (name, tensor, shape) of ``wanted`` that has a tensor: contiguous, of ``dtype``, on device ``here`` and of that
+    shape (None: any). One pass of cheap comparisons: an operator of a few microseconds takes up to fifteen tensors."""
+    for name, tensor, shape in wanted:
         if tensor is None:
             continue
-        if not tensor.is_cuda:
-            raise KernelLibraryError(f"{name} must be a CUDA tensor (there is no CPU path)")
-        if tensor.device.index != here or (_device_index is not None and here != _device_index):
-            raise KernelLibraryError(f"{name} is on {tensor.device}, kernels run on cuda:{here if _device_index is None else _device_index}")
-
-
-def _need_ints(name: str, tensor: torch.Tensor | None, *shape: int) -> None:
-    """``tensor`` (where there is one): contiguous int32 of that shape, -1 for any size."""
-    if tensor is None:
-        return
-    _need(tensor, name, torch.int32)
-    if tensor.ndim != len(shape) or any(want >= 0 and have != want for have, want in zip(tensor.shape, shape)):
-        raise KernelLibraryError(f"{name} must be int32 {list(shape)}, got {list(tensor.shape)}")
+        if tensor.dtype is not dtype or tensor.get_device() != here or not tensor.is_contiguous() or (
+                shape is not None and tensor.shape != shape):
+            _need(tensor, name, dtype)
+            if tensor.get_device() != here:
+                raise KernelLibraryError(f"{name} is on {tensor.device}, kernels run on cuda:{here}")
+            raise KernelLibraryError(f"{name} must be {dtype} {list(shape)}, got {list(tensor.shape)}")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -716,19 +721,16 @@ def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, 
     up to rounding. All three are host numbers, so that a captured step can be replayed with other lengths and groups
     below them. ``scratch`` (float32) is taken from torch's allocator where none is given. The keys and values that any
     token of a group sees have to be finite."""
-    _need(q, "q", contiguous=False)
-    _need(cache, "cache", q.dtype)
-    _need(out, "out", q.dtype, contiguous=False)
-    _need_here(("q", q), ("cache", cache), ("block_tables", block_tables), ("cu_q", cu_q), ("context_lens", context_lens),
-               ("tok_seq", tok_seq), ("positions", positions), ("shared_first", shared_first), ("shared_lens", shared_lens),
-               ("out", out), ("status", status), ("sink", sink), ("scratch", scratch))
-    code = dtype_code(q.dtype)
-    n_seqs = context_lens.numel()
-    for name, tensor, shape in (("context_lens", context_lens, (n_seqs,)), ("block_tables", block_tables, (n_seqs, -1)),
-                                ("cu_q", cu_q, (n_seqs + 1,)), ("tok_seq", tok_seq, (-1,)), ("positions", positions, (-1,)),
-                                ("shared_first", shared_first, (-1,)), ("shared_lens", shared_lens, (n_seqs,))):
-        _need_ints(name, tensor, *shape)
-    _need(status, "status", torch.int32)
+    here, code = _here("q", q), dtype_code(q.dtype)
+    n_seqs, int32 = context_lens.numel(), torch.int32
+    _need_all(here, q.dtype, ("cache", cache, None))
+    _need_all(here, int32, ("context_lens", context_lens, (n_seqs,)), ("block_tables", block_tables, None), ("cu_q", cu_q, (n_seqs + 1,)),
+              ("tok_seq", tok_seq, None), ("positions", positions, None), ("shared_first", shared_first, None),
+              ("shared_lens", shared_lens, (n_seqs,)), ("status", status, None))
+    if out.dtype is not q.dtype or out.get_device() != here:
+        raise KernelLibraryError(f"out must be {q.dtype} on {q.device}, got {out.dtype} on {out.device}")
+    if block_tables.ndim != 2 or block_tables.shape[0] != n_seqs:
+        raise KernelLibraryError(f"block_tables must hold a row for each of {n_seqs} sequences, got {list(block_tables.shape)}")
     n_groups = shared_first.numel() - 1
     if n_groups < 1 and n_seqs > 0:
         raise KernelLibraryError("shared_first must hold the start of at least one group and the end of the last")
@@ -749,7 +751,8 @@ def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, 
                                      int(max_q_len), int(max_shared_len), int(max_own_len), n_sm)
     if scratch is None:
         scratch = torch.empty((need + 3) // 4, dtype=torch.float32, device=q.device)
-    _need(scratch, "scratch", torch.float32)
+    else:
+        _need_all(here, torch.float32, ("scratch", scratch, None))
     if scratch.numel() * 4 < need or scratch.data_ptr() % 16 != 0:
         raise KernelLibraryError(f"attention over shared keys needs {need} bytes of 16-byte aligned scratch")
     check(library().mx_paged_attention_shared(
@@ -780,18 +783,19 @@ def step_tables(q_lens: torch.Tensor, context_lens: torch.Tensor, rows: torch.Te
     ``context_lens[s]`` on sees: ``window`` and ``keep_first`` as in ``paged_attention``, a negative window for blocks. Lengths and
     free pages are only read, so the same step may be laid out again. A step that does not fit sets the status word and
     comes out empty, with ``tables`` as they were; of two sequences with one row the later one does."""
-    tensors = (("q_lens", q_lens), ("context_lens", context_lens), ("rows", rows), ("tables", tables), ("free_pages", free_pages),
-               ("n_free", n_free), ("positions", positions), ("tok_seq", tok_seq), ("cu_q", cu_q), ("slots", slots),
-               ("block_tables", block_tables), ("taken", taken), ("status", status), ("shared_rows", shared_rows),
-               ("shared_pages", shared_pages))
-    _need_here(*tensors)
+    here = _here("q_lens", q_lens)
     n_seqs, n_tokens = q_lens.numel(), positions.numel()
-    width = tables.shape[-1]
-    shapes = {"q_lens": (n_seqs,), "context_lens": (n_seqs,), "rows": (n_seqs,), "tables": (-1, -1), "free_pages": (-1,),
-              "n_free": (1,), "positions": (-1,), "tok_seq": (n_tokens,), "cu_q": (n_seqs + 1,), "slots": (n_tokens,),
-              "block_tables": (n_seqs, width), "taken": (1,), "status": (1,), "shared_rows": (n_seqs,), "shared_pages": (n_seqs,)}
-    for name, tensor in tensors:
-        _need_ints(name, tensor, *shapes[name])
+    if tables.ndim != 2:
+        raise KernelLibraryError(f"tables must be [table rows, width], got {list(tables.shape)}")
+    width = tables.shape[1]
+    per_seq, per_token = (n_seqs,), (n_tokens,)
+    _need_all(here, torch.int32, ("q_lens", q_lens, per_seq), ("context_lens", context_lens, per_seq), ("rows", rows, per_seq),
+              ("tables", tables, None), ("free_pages", free_pages, None), ("n_free", n_free, None), ("positions", positions, per_token),
+              ("tok_seq", tok_seq, per_token), ("cu_q", cu_q, (n_seqs + 1,)), ("slots", slots, per_token),
+              ("block_tables", block_tables, (n_seqs, width)), ("taken", taken, None), ("status", status, None),
+              ("shared_rows", shared_rows, per_seq), ("shared_pages", shared_pages, per_seq))
+    if n_free.numel() < 1 or taken.numel() < 1 or status.numel() < 1:
+        raise KernelLibraryError("n_free, taken and status hold a number each")
     if rows is None and tables.shape[0] < n_seqs:
         raise KernelLibraryError(f"{n_seqs} sequences need as many rows of tables, got {tables.shape[0]}")
     check(library().mx_step_tables(
@@ -803,6 +807,11 @@ def step_tables(q_lens: torch.Tensor, context_lens: torch.Tensor, rows: torch.Te
 
 
 # ---------------------------------------------------------------------- scores before a token is drawn
+@functools.lru_cache(maxsize=4096)
+def _adjust_logits_scratch(*sizes: int) -> int:
+    return int(library().mx_adjust_logits_scratch(*sizes))
+
+
 def adjust_logits(logits: torch.Tensor, out: torch.Tensor, token_offsets: torch.Tensor | None = None,
                   token_ids: torch.Tensor | None = None, repeat_penalty: torch.Tensor | None = None,
                   presence_penalty: torch.Tensor | None = None, frequency_penalty: torch.Tensor | None = None, *,
@@ -820,32 +829,26 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, token_offsets: torch.
     token v may be taken; a score that may not becomes -infinity. Row r goes by mask ``mask_rows[r]`` (-1: none), or by
     mask r where there is no ``mask_rows``. Ids outside the vocabulary are passed over. Rows of ``logits`` and ``out`` may be
     strided."""
-    tensors = (("token_offsets", token_offsets), ("token_ids", token_ids), ("bias_offsets", bias_offsets), ("bias_ids", bias_ids),
-               ("mask_words", mask_words), ("mask_rows", mask_rows), ("pending_ids", pending_ids))
-    floats = (("repeat_penalty", repeat_penalty), ("presence_penalty", presence_penalty), ("frequency_penalty", frequency_penalty),
-              ("bias_values", bias_values))
-    _need(logits, "logits", contiguous=False)
-    _need(out, "out", torch.float32, contiguous=False)
-    _need_here(("logits", logits), ("out", out), *tensors, *floats)
-    code = dtype_code(logits.dtype)
+    here, code = _here("logits", logits), dtype_code(logits.dtype)
+    if out.dtype is not torch.float32 or out.get_device() != here:
+        raise KernelLibraryError(f"out must be float32 on {logits.device}, got {out.dtype} on {out.device}")
     if logits.ndim != 2 or logits.shape != out.shape or logits.stride(1) != 1 or out.stride(1) != 1:
         raise KernelLibraryError(f"logits and out must be [rows, vocab] with neighbouring columns, got {list(logits.shape)} and {list(out.shape)}")
     n_rows, vocab = logits.shape
     if n_rows > 1 and out.stride(0) < vocab:
         raise KernelLibraryError("rows of out must not overlap")
-    shapes = {"token_offsets": (n_rows + 1,), "token_ids": (-1,), "bias_offsets": (n_rows + 1,), "bias_ids": (-1,),
-              "mask_words": (-1, -1), "mask_rows": (n_rows,), "pending_ids": (n_rows,)}
-    for name, tensor in tensors:
-        _need_ints(name, tensor, *shapes[name])
-    for name, tensor in floats:
-        if tensor is not None:
-            _need(tensor, name, torch.float32)
-            if name != "bias_values" and tensor.shape != (n_rows,):
-                raise KernelLibraryError(f"{name} must be float32 [{n_rows}], got {list(tensor.shape)}")
+    per_row, ends = (n_rows,), (n_rows + 1,)
+    _need_all(here, torch.int32, ("token_offsets", token_offsets, ends), ("token_ids", token_ids, None), ("bias_offsets", bias_offsets, ends),
+              ("bias_ids", bias_ids, None), ("mask_words", mask_words, None), ("mask_rows", mask_rows, per_row),
+              ("pending_ids", pending_ids, per_row))
+    _need_all(here, torch.float32, ("repeat_penalty", repeat_penalty, per_row), ("presence_penalty", presence_penalty, per_row),
+              ("frequency_penalty", frequency_penalty, per_row), ("bias_values", bias_values, None))
+    if mask_words is not None and mask_words.ndim != 2:
+        raise KernelLibraryError(f"mask_words must be [masks, words], got {list(mask_words.shape)}")
     if (token_offsets is None) != (token_ids is None):
         raise KernelLibraryError("token_offsets and token_ids go together")
-    if len({bias_offsets is None, bias_ids is None, bias_values is None}) > 1 or (
-            bias_ids is not None and bias_ids.shape != bias_values.shape):
+    if not (bias_offsets is None) == (bias_ids is None) == (bias_values is None) or (
+            bias_ids is not None and bias_ids.numel() != bias_values.numel()):
         raise KernelLibraryError("bias_offsets, bias_ids and bias_values go together, a value an id")
     if mask_words is None and mask_rows is not None or mask_words is not None and mask_rows is None and mask_words.shape[0] != n_rows:
         raise KernelLibraryError("mask_rows says which of mask_words' rows a row of scores goes by; without it there is one each")
@@ -859,12 +862,15 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, token_offsets: torch.
         if code != F32 or n_rows > 1 and stride != logits.stride(0) or not (
                 out.data_ptr() == first or n_rows > 1 and vocab <= apart <= stride - vocab):
             raise KernelLibraryError("out lies over a part of logits; it may be the same rows, or others")
+    n_ids = 0 if token_ids is None else token_ids.numel()
+    need = _adjust_logits_scratch(n_ids, n_rows, vocab)
+    scratch = torch.empty(need // 4, dtype=torch.int32, device=logits.device) if need else None
     check(library().mx_adjust_logits(
-        _ptr(logits), code, logits.stride(0), _ptr(out), out.stride(0), n_rows, vocab, _ptr(token_offsets), _ptr(token_ids),
+        _ptr(logits), code, logits.stride(0), _ptr(out), out.stride(0), n_rows, vocab, _ptr(token_offsets), _ptr(token_ids), n_ids,
         _ptr(repeat_penalty), _ptr(presence_penalty), _ptr(frequency_penalty), _ptr(bias_offsets), _ptr(bias_ids), _ptr(bias_values),
         _ptr(mask_words), 0 if mask_words is None else mask_words.shape[0], 0 if mask_words is None else mask_words.shape[1],
-        _ptr(mask_rows), _ptr(pending_ids), _stream()), "adjust_logits")
-    _launched()
+        _ptr(mask_rows), _ptr(pending_ids), _ptr(scratch), _stream()), "adjust_logits")
+    _launched(2 if need else 1)
 
 
 # ---------------------------------------------------------------------- RMS norm, post-norm sums

@@ -174,8 +174,9 @@ def test_padding_sequences_bring_nothing():
     assert case.run() == expected and case.status.item() == 0
 
 
-def test_tables_wider_than_a_blocks_share():
-    case = Case([1, 3], [70000, 10], 16, width=9000).device()
+@pytest.mark.parametrize("width", [9000, 40000])
+def test_tables_wider_than_a_blocks_share(width):
+    case = Case([1, 3], [70000, 10], 16, width=width).device()
     assert case.run() == case.expected() and case.status.item() == 0
 
 
