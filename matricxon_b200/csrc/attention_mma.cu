@@ -271,7 +271,7 @@ attention_mma_kernel(const MmaAttnParams p) {
     } else if (KEYS == OWN_KEYS && !NARROW) {
         const SequenceTile found = find_sequence_tile(p.cu_q, p.shared.n_seqs, tile, TILE_ROWS, p.group, lane);
         if (found.seq < 0) {
-            pdl_wait();
+            wait_for_shared_keys();
             return;
         }
         seq = found.seq; tile_row0 = found.row;
@@ -279,7 +279,7 @@ attention_mma_kernel(const MmaAttnParams p) {
         seq = p.tiles ? p.tiles[2 * tile] : tile;
         tile_row0 = p.tiles ? p.tiles[2 * tile + 1] : 0;
     }
-    if (NARROW) {
+    if (NARROW && KEYS == ALL_KEYS) {
         // the block-table row sets out together with the sequence's lengths (it does not depend on
         // them): one trip to memory instead of two before the first page can be asked for
         const int* row = p.block_tables + (size_t)seq * p.bt_stride;
@@ -294,7 +294,8 @@ attention_mma_kernel(const MmaAttnParams p) {
     const int own_from = KEYS == OWN_KEYS && p.shared.lens != nullptr ? p.shared.lens[seq] : 0;
     const int n_rows = q_len * group;
     if (tile_row0 >= n_rows) {                  // a padding sequence of a fixed-size batch
-        if (p.beside || KEYS == OWN_KEYS) pdl_wait();   // a block that ends has let the next kernel start
+        if (p.beside) pdl_wait();               // a block that ends has let the next kernel start
+        if (KEYS == OWN_KEYS) wait_for_shared_keys();
         return;
     }
     if (KEYS == OWN_KEYS && NARROW && n_rows > TILE_ROWS && tid == 0)
@@ -373,6 +374,12 @@ attention_mma_kernel(const MmaAttnParams p) {
     auto chunk_of = [&](int v) { return v < n_kept ? v : first_chunk + v - n_kept; };
 
     const int* bt = p.block_tables + (size_t)seq * p.bt_stride;
+    // a sequence's own keys begin far into its row, behind the shared ones
+    const int table_from = KEYS == OWN_KEYS ? first_chunk * (CHUNK >> p.page_shift) : 0;
+    if (NARROW && KEYS == OWN_KEYS) {
+        for (int e = tid; e < min(p.bt_stride - table_from, NARROW_TABLE); e += 32 * N_WARPS) narrow_table[e] = bt[table_from + e];
+        __syncthreads();
+    }
     const size_t head_stride = (size_t)p.page_size * HD;
     const size_t page_stride = 2 * (size_t)p.n_kv_heads * head_stride;
     const __nv_bfloat16* kbase = p.cache + (size_t)kh * head_stride;
@@ -390,7 +397,7 @@ attention_mma_kernel(const MmaAttnParams p) {
     auto cached_for = [&](int i) -> const int* {
         const int pages = CHUNK >> p.page_shift;
         const int first = chunk_of(my_first + N_WARPS * i) * pages;
-        return first + pages <= min(p.bt_stride, NARROW_TABLE) ? narrow_table + first : nullptr;
+        return first + pages <= p.bt_stride && first + pages <= table_from + NARROW_TABLE ? narrow_table + (first - table_from) : nullptr;
     };
     const bool first_is_old = (chunk_of(my_first) + 1) * CHUNK <= ctx;
     if (NARROW && my_count > 0 && first_is_old)
@@ -717,7 +724,7 @@ attention_mma_kernel(const MmaAttnParams p) {
             p.part_ml[base * 2] = max_of[tid] * ln2;     // the merge kernel works with natural logs
             p.part_ml[base * 2 + 1] = sum_of[tid];
         }
-        if (KEYS == OWN_KEYS) pdl_wait();                // whoever waits for this kernel waits for the shared keys' too
+        if (KEYS == OWN_KEYS) wait_for_shared_keys();
         return;
     }
 
@@ -785,7 +792,7 @@ attention_mma_kernel(const MmaAttnParams p) {
             }
         }
     }
-    if (KEYS == OWN_KEYS) pdl_wait();
+    if (KEYS == OWN_KEYS) wait_for_shared_keys();
 }
 
 template <int HD, bool NARROW, bool BIASED, Keys KEYS>

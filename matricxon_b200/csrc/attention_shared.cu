@@ -103,7 +103,7 @@ shared_simt_kernel(const SharedAttnParams p) {
         rows = min(SH_ROWS, p.group - first_row);
         seq = first_token < p.cu_q[p.shared.n_seqs] ? p.shared.tok_seq[first_token] : -1;
         if (seq < 0 || seq >= p.shared.n_seqs) {
-            pdl_wait();
+            wait_for_shared_keys();
             return;
         }
     }
@@ -278,7 +278,7 @@ shared_simt_kernel(const SharedAttnParams p) {
             }
             if (tid == 0) { p.part_ml[base * 2] = row_m[r]; p.part_ml[base * 2 + 1] = row_l[r]; }
         }
-    if (!SHARED) pdl_wait();                 // whoever waits for this kernel waits for the shared keys' too
+    if (!SHARED) wait_for_shared_keys();
 }
 
 // The join: a warp a (token, head), four dimensions a lane. A token of no sequence is left alone.
@@ -371,6 +371,21 @@ struct SharedPlan {
     bool narrow;
 };
 
+// The number of parts, at most 32, that `blocks` blocks of `chunks` chunks each are cut into. `start`: what a block costs beside
+// its chunks, in chunks. `uneven`: the blocks' chunks differ, up to that many; they then go on one after another, half as long
+// on the average.
+int best_parts(long long blocks, int chunks, int room, int start, int uneven) {
+    int best = 1;
+    long long least = 0;
+    for (int parts = 1; parts <= 32 && parts <= chunks; ++parts) {
+        const int each = (chunks + parts - 1) / parts;
+        const long long rounds = (blocks * parts + room - 1) / room;
+        const long long cost = uneven ? blocks * parts * (each / 2 + start) / room + each + start : rounds * (each + start);
+        if (parts == 1 || cost < least) { best = parts; least = cost; }
+    }
+    return best;
+}
+
 SharedPlan make_plan(int dtype, int head_dim, int page_size, bool aligned, int n_tokens, int n_heads, int n_kv_heads, int n_seqs,
                      int n_groups, int max_q_len, int max_shared_len, int max_own_len, int n_sm) {
     SharedPlan plan;
@@ -384,14 +399,13 @@ SharedPlan make_plan(int dtype, int head_dim, int page_size, bool aligned, int n
     const int shared_rows = tc ? 128 / group * group : (mma ? 64 : SH_ROWS);
     plan.shared_tiles = (int)min(rows / shared_rows + n_groups, rows);
     plan.own_tiles = mma ? (plan.narrow ? n_seqs : (int)min(rows / 64 + n_seqs, rows)) : n_tokens * ((group + SH_ROWS - 1) / SH_ROWS);
-    // A share of the shared keys a block is worth it from two chunks on (128 keys with tcgen05, a block an SM; else 32, four an
-    // SM); the own keys' from four chunks a block (its four warps take one each; wide tiles two pairs), or two. With few tiles
-    // the parts fill the GPU; with many they only even out.
+    // Parts: blocks run in rounds of as many as fit the GPU (tcgen05 one an SM, narrow tiles two, the others three), and a round
+    // takes as long as a block's chunks and its start. The number of parts with the shortest rounds is taken; the tiles of a
+    // group each end in the middle of one, so there may be a tile a group more.
     const int shared_chunks = (max(max_shared_len, 1) + (tc ? 127 : 31)) / (tc ? 128 : 32), own_chunks = max(max_own_len, 1) / 32 + 1;
     const long long shared_blocks = (rows + shared_rows - 1) / shared_rows * n_kv_heads, own_blocks = (long long)plan.own_tiles * n_kv_heads;
-    const long long room = tc ? n_sm : 4 * n_sm, own_room = plan.narrow ? 2 * n_sm : 4 * n_sm;
-    plan.shared_parts = max_shared_len <= 0 ? 0 : (int)max(1LL, min(min(room / max(shared_blocks, 1LL), (long long)shared_chunks / 2), 32LL));
-    plan.own_parts = (int)max(1LL, min(min(own_room / max(own_blocks, 1LL), (long long)own_chunks / (plan.narrow ? 4 : 2)), 32LL));
+    plan.shared_parts = max_shared_len <= 0 ? 0 : best_parts(shared_blocks, shared_chunks, tc ? n_sm : 3 * n_sm, tc ? 4 : 8, 0);
+    plan.own_parts = best_parts(own_blocks, (own_chunks + 3) / 4, plan.narrow ? 2 * n_sm : 3 * n_sm, 3, 1);
     return plan;
 }
 

@@ -19,6 +19,13 @@ struct SharedPrefixParams {
     int beside;              // the kernel of the shared keys was launched just before this one, which begins beside it
 };
 
+// At the end of a block of the kernel of the own keys, which began beside that of the shared ones: the grid must not be done
+// before the other is, since what comes next waits for this one. One block that waits is enough (with all of them waiting,
+// those that are done hold the SMs of those that have not begun).
+__device__ __forceinline__ void wait_for_shared_keys() {
+    if ((blockIdx.x | blockIdx.y | blockIdx.z) == 0) pdl_wait();
+}
+
 struct KeyRange {
     int first, last;         // none: last < first
 };

@@ -26,6 +26,7 @@ namespace {
 
 constexpr int ST_THREADS = 512;
 constexpr int ST_OWN = 64;              // sequences a block lays out, at most
+constexpr int ST_AHEAD = 8;
 constexpr int ST_SLICE = 16384;         // block-table entries of a sequence that one block writes
 
 struct StepTablesParams {
@@ -37,7 +38,7 @@ struct StepTablesParams {
 
 struct Sequence {
     int q, context, row, shared_row, shared;      // shared: pages
-    int have, need;
+    int have, need, seen_from;                    // pages held, taken, and the first one that the next query needs
     bool fits;                                    // its numbers are possible
 };
 
@@ -59,6 +60,7 @@ __device__ __forceinline__ Sequence read_sequence(const StepTablesParams& p, int
     // (sums of two numbers below 2^31 and a page fit 32 bits without a sign)
     v.have = (int)(((unsigned)v.context + (unsigned)p.page_size - 1u) / (unsigned)p.page_size);
     v.need = (int)(((unsigned)v.context + (unsigned)v.q + (unsigned)p.page_size - 1u) / (unsigned)p.page_size) - v.have;
+    v.seen_from = (int)((unsigned)first_visible_key(v.context, p.window) / (unsigned)p.page_size);
     return v;
 }
 
@@ -66,7 +68,7 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTable
     __shared__ long long warp_total[ST_THREADS / 32];
     __shared__ int warp_sums[3][ST_THREADS / 32];
     __shared__ Sequence own[ST_OWN];
-    __shared__ int repeated[ST_OWN];
+    __shared__ int repeated[ST_OWN], own_row[ST_OWN], own_page[ST_OWN];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int first = blockIdx.x * p.per_block, last = min(p.n_seqs, first + p.per_block);
     pdl_wait();
@@ -121,59 +123,80 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTable
         if (!possible) atomicOr(p.status, MX_STATUS_BAD_STEP);
     }
 
-    // ---- this block's sequences
-    const int k_begin = blockIdx.y * ST_SLICE, k_end = min(p.width, k_begin + ST_SLICE);
-    int begin_next = q_before, taken_next = need_before;
-    for (int s = first; s < last; ++s) {
-        const Sequence v = own[s - first];
-        const int begin = begin_next, taken = taken_next;
-        begin_next += v.q;
-        taken_next += v.need;
-        const bool there = possible && v.row >= 0 && !repeated[s - first];
-        if (blockIdx.y == 0 && tid == 0) {
-            p.cu_q[s + 1] = possible ? begin + v.q : 0;
-            if (possible && repeated[s - first]) atomicOr(p.status, MX_STATUS_BAD_STEP);
-        }
-        int* mine = p.tables + (size_t)max(v.row, 0) * p.width;
-        const int* leader = p.tables + (size_t)max(v.shared_row, 0) * p.width;
-        const int end = there ? v.have + v.need : 0;
-        // pages that nobody sees any more: between the kept ones and the first that the next query needs
-        const int kept = p.window > 0 ? (p.keep_first + p.page_size - 1) / p.page_size : 0;
-        const int seen_from = first_visible_key(v.context, p.window) / p.page_size;
-        int* out = p.block_tables + (size_t)s * p.width;
-        bool bad_page = false;
-#pragma unroll 8
-        for (int k = k_begin + tid; k < k_end; k += ST_THREADS) {
-            int page = -1;
-            if (k < end) {
-                const bool is_new = k >= v.have;
-                page = is_new ? p.free_pages[taken + k - v.have] : (k < v.shared ? leader[k] : mine[k]);
-                const bool seen = k < kept || k >= seen_from;
-                if (is_new) mine[k] = page;
-                if (!seen) page = -1;
-                else if (page < 0 || page >= p.n_pages) {
-                    page = -1;
-                    bad_page = true;
-                }
-            }
-            out[k] = page;
-        }
-        if (bad_page) atomicOr(p.status, MX_STATUS_BAD_PAGE);
-        if (blockIdx.y == 0 && possible) {
-            for (int i = tid; i < v.q; i += ST_THREADS) {
-                const int position = v.context + i, k = position / p.page_size;
-                int slot = -1;
-                if (there) {
-                    const int page = k >= v.have ? p.free_pages[taken + k - v.have] : mine[k];
-                    if (page >= 0 && page < p.n_pages) slot = page * p.page_size + position % p.page_size;
-                    else atomicOr(p.status, MX_STATUS_BAD_PAGE);
-                }
-                p.positions[begin + i] = there ? position : 0;
-                p.tok_seq[begin + i] = there ? s : -1;
-                p.slots[begin + i] = slot;
-            }
+    // ---- this block's sequences: where each one's rows and new pages begin, then their tables' entries, all in one row
+    const int mine_n = last - first;
+    if (tid < mine_n) {
+        int rows_before = q_before, pages_before = need_before;
+        for (int i = 0; i < tid; ++i) { rows_before += own[i].q; pages_before += own[i].need; }
+        own_row[tid] = rows_before;
+        own_page[tid] = pages_before;
+        if (blockIdx.y == 0) {
+            p.cu_q[first + tid + 1] = possible ? rows_before + own[tid].q : 0;
+            if (possible && repeated[tid]) atomicOr(p.status, MX_STATUS_BAD_STEP);
         }
     }
+    __syncthreads();
+    // pages that nobody sees any more lie between the kept ones and the first that the next query needs
+    const int kept = p.window > 0 ? (p.keep_first + p.page_size - 1) / p.page_size : 0;
+    const int k_begin = blockIdx.y * ST_SLICE, k_end = min(p.width, k_begin + ST_SLICE);
+    bool bad_page = false;
+    for (int i = 0; i < mine_n; ++i) {
+        const Sequence v = own[i];
+        const bool there = possible && v.row >= 0 && !repeated[i];
+        const int end = there ? min(k_end, v.have + v.need) : 0;
+        int* out = p.block_tables + (size_t)(first + i) * p.width;
+        int* row = p.tables + (size_t)max(v.row, 0) * p.width;
+        const int* leader = p.tables + (size_t)max(v.shared_row, 0) * p.width;
+        const int* fresh = p.free_pages + own_page[i] - v.have;
+        // eight entries a thread are asked for before one is written: the rows are read and written in one place
+        for (int k0 = k_begin + tid; k0 < end; k0 += ST_AHEAD * ST_THREADS) {
+            int page[ST_AHEAD];
+#pragma unroll
+            for (int u = 0; u < ST_AHEAD; ++u) {
+                const int k = k0 + u * ST_THREADS;
+                page[u] = k >= end ? -1 : (k >= v.have ? fresh[k] : (k < v.shared ? leader[k] : row[k]));
+            }
+#pragma unroll
+            for (int u = 0; u < ST_AHEAD; ++u) {
+                const int k = k0 + u * ST_THREADS;
+                if (k >= end) break;
+                if (k >= v.have) row[k] = page[u];
+                if (k >= kept && k < v.seen_from) page[u] = -1;
+                else if (page[u] < 0 || page[u] >= p.n_pages) {
+                    page[u] = -1;
+                    bad_page = true;
+                }
+                out[k] = page[u];
+            }
+        }
+#pragma unroll 8
+        for (int k = max(k_begin, end) + tid; k < k_end; k += ST_THREADS) out[k] = -1;
+    }
+    if (blockIdx.y == 0 && possible) {
+        // their token rows, a warp a sequence of few (decoding requests), the block one of more
+        auto token_rows = [&](int i, int r0, int step) {
+            const Sequence& v = own[i];
+            const bool there = !repeated[i];
+            for (int r = r0; r < v.q; r += step) {
+                const int position = v.context + r, k = (int)((unsigned)position / (unsigned)p.page_size);
+                int slot = -1;
+                if (there) {
+                    const int page = k >= v.have ? p.free_pages[own_page[i] + k - v.have] : p.tables[(size_t)v.row * p.width + k];
+                    if (page >= 0 && page < p.n_pages) slot = page * p.page_size + position - k * p.page_size;
+                    else bad_page = true;
+                }
+                const int t = own_row[i] + r;
+                p.positions[t] = there ? position : 0;
+                p.tok_seq[t] = there ? first + i : -1;
+                p.slots[t] = slot;
+            }
+        };
+        for (int i = warp; i < mine_n; i += ST_THREADS / 32)
+            if (own[i].q <= 32) token_rows(i, lane, 32);
+        for (int i = 0; i < mine_n; ++i)
+            if (own[i].q > 32) token_rows(i, tid, ST_THREADS);
+    }
+    if (bad_page) atomicOr(p.status, MX_STATUS_BAD_PAGE);
     // ---- rows behind the last token
     if (blockIdx.y == 0)
         for (int t = total + blockIdx.x * ST_THREADS + tid; t < p.n_tokens; t += gridDim.x * ST_THREADS) {
@@ -193,7 +216,7 @@ extern "C" int mx_step_tables(const int* q_lens, const int* context_lens, const 
     if (n_seqs <= 0) MX_REFUSE("step tables: a step of %d sequences", n_seqs);
     if (width <= 0 || n_rows <= 0 || n_tokens < 0) MX_REFUSE("step tables: %d rows of %d entries, %d tokens", n_rows, width, n_tokens);
     if (page_size <= 0) MX_REFUSE("step tables: pages of %d positions", page_size);
-    if ((long long)n_seqs * width > 0x7fffffffLL) MX_REFUSE("step tables: %d tables of %d entries", n_seqs, width);
+    if ((long long)n_seqs * width > 0x7fffffffLL || (long long)n_rows * width > 0x7fffffffffffLL) MX_REFUSE("step tables: %d tables of %d entries", n_seqs, width);
     if (n_pages <= 0 || n_pages * page_size > 0x7fffffffLL) MX_REFUSE("step tables: %lld pages of %d positions have no 32-bit slots", n_pages, page_size);
     if (keep_first < 0) MX_REFUSE("step tables: %d kept positions", keep_first);
     if ((shared_rows == nullptr) != (shared_pages == nullptr)) MX_REFUSE("step tables: shared rows and shared pages go together");
@@ -203,9 +226,9 @@ extern "C" int mx_step_tables(const int* q_lens, const int* context_lens, const 
     p.slots = slots; p.block_tables = block_tables; p.taken = taken; p.status = status;
     p.n_seqs = n_seqs; p.n_tokens = n_tokens; p.n_rows = n_rows; p.width = width; p.page_size = page_size; p.n_pages = (int)n_pages;
     p.n_free_most = n_free_most; p.window = window; p.keep_first = window > 0 ? keep_first : 0;
-    // a block a sequence while that makes no more than four blocks an SM
-    p.per_block = (n_seqs + 591) / 592;
-    if (p.per_block > ST_OWN) MX_REFUSE("step tables: %d sequences, at most %d a step", n_seqs, 592 * ST_OWN);
+    // a block a sequence while that makes no more than two blocks an SM: more of them add up the lengths more often
+    p.per_block = (n_seqs + 295) / 296;
+    if (p.per_block > ST_OWN) MX_REFUSE("step tables: %d sequences, at most %d a step", n_seqs, 296 * ST_OWN);
     const dim3 grid((n_seqs + p.per_block - 1) / p.per_block, (width + ST_SLICE - 1) / ST_SLICE);
     if (grid.y > 65535) MX_REFUSE("step tables: tables of %d entries a row", width);
     const cudaError_t e = mx_launch_chained(step_tables_kernel, grid, dim3(ST_THREADS), 0, stream, p);

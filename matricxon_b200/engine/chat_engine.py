@@ -72,6 +72,8 @@ class ChatEngine:
         vocab = self.model.spec.vocab_size
         if tokens and not (0 <= min(tokens) and max(tokens) < vocab):
             raise RequestRefused(f"the prompt holds a token id outside the vocabulary of {vocab}")
+        if sampling is not None and sampling.largest_token_id >= vocab:
+            raise RequestRefused(f"the sampling options name a token id outside the vocabulary of {vocab}")
         if request_id in self.scheduler.finished or self.core.cache.has_request(request_id) \
                 or any(s.request_id == request_id for s in self.scheduler.waiting):
             raise RequestRefused(f"request id {request_id!r} is already in use")

@@ -35,6 +35,8 @@ def build_parser() -> argparse.ArgumentParser:
     parser.add_argument("--top-k", type=int, default=40)
     parser.add_argument("--top-p", type=float, default=0.9)
     parser.add_argument("--repeat-penalty", type=float, default=1.1)
+    parser.add_argument("--presence-penalty", type=float, default=0.0)
+    parser.add_argument("--frequency-penalty", type=float, default=0.0)
     parser.add_argument("--seed", type=int, default=0)
     parser.add_argument("--eos-token-id", type=int, action="append", default=[])
     parser.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
@@ -84,7 +86,8 @@ def main(argv: list[str] | None = None) -> int:
                         max_active=1, max_batched_tokens=args.max_batched_tokens,
                         prefill_chunk=args.prefill_chunk, max_model_len=num_ctx)
     sampling = SamplingConfig(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
-                              repeat_penalty=args.repeat_penalty, num_ctx=num_ctx,
+                              repeat_penalty=args.repeat_penalty, presence_penalty=args.presence_penalty,
+                              frequency_penalty=args.frequency_penalty, num_ctx=num_ctx,
                               num_predict=args.num_predict, seed=args.seed)
     started = time.monotonic()
     result = engine.generate(GenerationRequest(input_ids=prompt, sampling=sampling))

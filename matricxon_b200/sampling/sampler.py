@@ -45,6 +45,7 @@ class RequestSampler:
         self.generated: list[int] = []
         self._distinct: set[int] = set()
         self._distinct_list: list[int] = []
+        self._mask_words: np.ndarray | None = None
 
     def next_uniform(self, ahead: int = 0) -> float:
         """The uniform of the next token, or of the one ``ahead`` tokens after it."""
@@ -57,9 +58,20 @@ class RequestSampler:
             self._distinct_list.append(token)
 
     def penalty_ids(self) -> list[int]:
-        if self.config.repeat_penalty == 1.0:
+        """The generated ids that the sampling kernel penalises: none where their scores were adjusted before it."""
+        if self.config.repeat_penalty == 1.0 or self.config.adjusts_scores:
             return []
         return self._distinct_list
+
+    def mask_words(self, vocab_size: int) -> np.ndarray | None:
+        """The allowed tokens as int32 words of a bit a token, None where all are allowed."""
+        if self.config.allowed_token_ids is None:
+            return None
+        if self._mask_words is None or self._mask_words.shape[0] != (vocab_size + 31) // 32:
+            bits = np.zeros((vocab_size + 31) // 32 * 32, dtype=np.uint8)
+            bits[list(self.config.allowed_token_ids)] = 1
+            self._mask_words = np.packbits(bits, bitorder="little").view("<i4")
+        return self._mask_words
 
 
 class BatchSampler:
@@ -69,6 +81,7 @@ class BatchSampler:
         self.device = torch.device(device)
         self.vocab_size = vocab_size
         self._work: torch.Tensor | None = None
+        self._adjusted: torch.Tensor | None = None
         self._params_host: torch.Tensor | None = None
         self._params_dev: torch.Tensor | None = None
         self._params_done: torch.cuda.Event | None = None
@@ -110,17 +123,25 @@ class BatchSampler:
             ids.extend(s.penalty_ids())
             offsets.append(len(ids))
         total = 4 * n + n + (n + 1) + len(ids)
+        # rows whose scores are adjusted first (adjust_logits) bring what that takes behind the rest of the buffer
+        adjusting = [s.config.adjusts_scores for s in samplers]
+        extra, places = self._adjustments(samplers, total) if any(adjusting) else (None, None)
+        plain = total
+        if extra is not None:
+            total += extra.shape[0]
         packed = np.empty(total, dtype=np.int32)
         as_float = packed[:4 * n].view(np.float32)
         as_float[0:n] = [s.config.temperature for s in samplers]
         as_float[n:2 * n] = [s.config.top_p for s in samplers]
-        as_float[2 * n:3 * n] = [s.config.repeat_penalty for s in samplers]
+        as_float[2 * n:3 * n] = [1.0 if adjusted else s.config.repeat_penalty for s, adjusted in zip(samplers, adjusting)]
         ahead = 0 if pending is None else 1
         as_float[3 * n:4 * n] = [s.next_uniform(ahead) for s in samplers]
         packed[4 * n:5 * n] = [s.config.top_k for s in samplers]
         packed[5 * n:6 * n + 1] = offsets
         if ids:
-            packed[6 * n + 1:] = ids
+            packed[6 * n + 1:plain] = ids
+        if extra is not None:
+            packed[plain:] = extra
         if self._params_host is None or self._params_host.numel() < total:
             size = max(total, 4096)
             self._params_host = torch.empty(size, dtype=torch.int32, pin_memory=True)
@@ -137,6 +158,8 @@ class BatchSampler:
         base = self._params_dev.data_ptr()
         if pending is not None and (pending.dtype != torch.int32 or not pending.is_cuda or pending.numel() < n):
             raise ValueError("pending ids must be int32 on the device, one per row")
+        if extra is not None:
+            logits = self._adjust(logits, places, pending)
         check(library().mx_sample(
             logits.data_ptr(), logits.stride(0), n, self.vocab_size,
             base, base + 4 * (4 * n), base + 4 * n, base + 4 * (2 * n), base + 4 * (3 * n),
@@ -155,6 +178,59 @@ class BatchSampler:
         done.record()
         self._device_ids[self._turn] = out
         return host, done, n
+
+    def _adjustments(self, samplers: list[RequestSampler], base: int) -> tuple[np.ndarray, dict]:
+        """What ``adjust_logits`` takes for these rows in one int32 array, and where each of its arguments lies in a
+        buffer that holds the array from ``base`` on: name -> (start, end, whether the bits are floats). A row that adjusts
+        nothing has penalties that change nothing and is left to the sampling kernel."""
+        tokens, token_offsets = [], [0]
+        biases, bias_offsets = [], [0]
+        masks, mask_rows = [], []
+        repeat, presence, frequency = [], [], []
+        for sampler in samplers:
+            config = sampler.config
+            adjusts = config.adjusts_scores
+            if adjusts and (config.repeat_penalty != 1.0 or config.presence_penalty or config.frequency_penalty):
+                tokens.extend(sampler.generated)
+            token_offsets.append(len(tokens))
+            repeat.append(config.repeat_penalty if adjusts else 1.0)
+            presence.append(config.presence_penalty)
+            frequency.append(config.frequency_penalty)
+            biases.extend(config.logit_bias)
+            bias_offsets.append(len(biases))
+            words = sampler.mask_words(self.vocab_size)
+            mask_rows.append(-1 if words is None else len(masks))
+            if words is not None:
+                masks.append(words)
+        pieces = [("token_offsets", token_offsets, False), ("token_ids", tokens, False), ("repeat_penalty", repeat, True),
+                  ("presence_penalty", presence, True), ("frequency_penalty", frequency, True)]
+        if biases:
+            pieces += [("bias_offsets", bias_offsets, False), ("bias_ids", [token for token, _ in biases], False),
+                       ("bias_values", [value for _, value in biases], True)]
+        if masks:
+            pieces += [("mask_rows", mask_rows, False), ("mask_words", np.concatenate(masks), False)]
+        arrays, places, at = [], {}, base
+        for name, values, is_float in pieces:
+            array = np.asarray(values, dtype=np.float32 if is_float else np.int32)
+            arrays.append(array.view(np.int32))
+            places[name] = (at, at + array.shape[0], is_float)
+            at += array.shape[0]
+        return np.concatenate(arrays), places
+
+    def _adjust(self, logits: torch.Tensor, places: dict, pending: torch.Tensor | None) -> torch.Tensor:
+        """The rows' scores with every penalty, bias and mask (the logits themselves stay as they are)."""
+        n = logits.shape[0]
+        if self._adjusted is None or self._adjusted.shape[0] < n:
+            self._adjusted = torch.empty((max(n, 8), self.vocab_size), dtype=torch.float32, device=self.device)
+        arguments = {}
+        for name, (start, end, is_float) in places.items():
+            part = self._params_dev[start:end]
+            arguments[name] = part.view(torch.float32) if is_float else part
+        if "mask_words" in arguments:
+            arguments["mask_words"] = arguments["mask_words"].view(-1, (self.vocab_size + 31) // 32)
+        out = self._adjusted[:n]
+        kernels.adjust_logits(logits, out, pending_ids=pending[:n] if pending is not None else None, **arguments)
+        return out
 
     def device_ids(self) -> torch.Tensor:
         """The ids of the latest ``launch`` on the device (int32 [rows])."""
