@@ -48,7 +48,8 @@ constexpr int MMA_WARPS = 4;        // wide tiles: 16 rows each
 constexpr int MMA_THREADS = MMA_WARPS * 32;
 constexpr int NARROW_WARPS = 8;     // narrow tiles: all warps hold the same rows and share the chunks
 constexpr int NARROW_THREADS = NARROW_WARPS * 32;
-constexpr int OWN_WARPS = 4;        // the same for OWN_KEYS
+constexpr int OWN_WARPS = 3;        // the same for OWN_KEYS: fewer warps, each with a chunk on its way while it works on another,
+constexpr int OWN_STAGES = 2;       // and two blocks an SM, so that one begins and ends while the other reads
 constexpr int CHUNK = 32;
 constexpr int WIDE_STAGES = 4;      // chunks in flight per block (two pairs), wide tiles
 constexpr int NARROW_STAGES = 1;    // chunks in flight per warp, narrow tiles
@@ -244,14 +245,15 @@ struct One { static constexpr int value = 1; };
 struct Two { static constexpr int value = 2; };
 
 template <int HD, bool NARROW, bool BIASED, Keys KEYS>
-__global__ void __launch_bounds__(NARROW && KEYS == ALL_KEYS ? NARROW_THREADS : MMA_THREADS, NARROW ? (KEYS == ALL_KEYS ? 1 : OWN_BLOCKS) : 3)
+__global__ void __launch_bounds__(NARROW ? (KEYS == ALL_KEYS ? NARROW_THREADS : 32 * OWN_WARPS) : MMA_THREADS, NARROW ? (KEYS == ALL_KEYS ? 1 : OWN_BLOCKS) : 3)
 attention_mma_kernel(const MmaAttnParams p) {
-    constexpr int N_WARPS = NARROW && KEYS == ALL_KEYS ? NARROW_WARPS : OWN_WARPS;   // of a narrow tile
+    constexpr int N_WARPS = KEYS == ALL_KEYS ? NARROW_WARPS : OWN_WARPS;             // of a narrow tile
+    constexpr int N_DEEP = KEYS == ALL_KEYS ? NARROW_STAGES : OWN_STAGES;            // chunks in flight of each of them
     constexpr int KB = HD / 32;                 // 32-wide blocks of the head dim
     constexpr int NB = HD / 8;                  // 8-wide output column blocks
     constexpr int STAGE_ELEMS = 2 * CHUNK * HD; // keys then values
     constexpr int TILE_ROWS = NARROW ? 16 : 16 * MMA_WARPS;
-    constexpr int N_STAGES = NARROW ? NARROW_STAGES * N_WARPS : WIDE_STAGES;
+    constexpr int N_STAGES = NARROW ? N_DEEP * N_WARPS : WIDE_STAGES;
     extern __shared__ __align__(128) unsigned char smem_raw[];
     __nv_bfloat16* stages = reinterpret_cast<__nv_bfloat16*>(smem_raw);
     __shared__ __align__(8) unsigned long long bars[N_STAGES];
@@ -388,8 +390,8 @@ attention_mma_kernel(const MmaAttnParams p) {
     // kernel), and the keys and values of positions before this step are in the cache since earlier
     // steps. So this warp's first chunk, if it holds none of this step's positions, sets out now, under
     // the tail of the kernel that computes the queries and the newest keys.
-    __nv_bfloat16* my_stages = stages + (size_t)(NARROW ? warp : 0) * NARROW_STAGES * STAGE_ELEMS;
-    unsigned long long* my_bars = bars + (NARROW ? warp : 0) * NARROW_STAGES;
+    __nv_bfloat16* my_stages = stages + (size_t)(NARROW ? warp : 0) * N_DEEP * STAGE_ELEMS;
+    unsigned long long* my_bars = bars + (NARROW ? warp : 0) * N_DEEP;
     const int my_first = c_begin + warp;
     const int my_count = NARROW && my_first < c_end ? (c_end - my_first + N_WARPS - 1) / N_WARPS : 0;
     // This warp's chunks find their pages in the row read ahead at the top (entries beyond what was
@@ -634,22 +636,22 @@ attention_mma_kernel(const MmaAttnParams p) {
             issue_chunk_warp<HD>(p, my_stages, my_stages + CHUNK * HD, &my_bars[0], chunk_of(my_first) * CHUNK, lo_tile,
                                  hi_tile, kept, bt, kbase, vbase, page_stride, lane, cached_for(0));
         for (int i = 0; i < my_count; ++i) {
-            const int st = i % NARROW_STAGES;
-            if (NARROW_STAGES > 1 && i + 1 < my_count) {
-                const int nx = (i + 1) % NARROW_STAGES;
+            const int st = i % N_DEEP;
+            if (N_DEEP > 1 && i + 1 < my_count) {
+                const int nx = (i + 1) % N_DEEP;
                 __nv_bfloat16* ks = my_stages + (size_t)nx * STAGE_ELEMS;
                 issue_chunk_warp<HD>(p, ks, ks + CHUNK * HD, &my_bars[nx], chunk_of(my_first + N_WARPS * (i + 1)) * CHUNK,
                                      lo_tile, hi_tile, kept, bt, kbase, vbase, page_stride, lane, cached_for(i + 1));
             }
             __syncwarp();
-            mbar_wait(&my_bars[st], (unsigned)((i / NARROW_STAGES) & 1), p.status);
+            mbar_wait(&my_bars[st], (unsigned)((i / N_DEEP) & 1), p.status);
             const __nv_bfloat16* ks = my_stages + (size_t)st * STAGE_ELEMS;
             {
                 const int c0 = chunk_of(my_first + N_WARPS * i) * CHUNK;
                 compute(One{}, ks, ks + CHUNK * HD, ks, ks + CHUNK * HD, c0, c0);
             }
             __syncwarp();                         // the stage may be refilled from here on
-            if (NARROW_STAGES == 1 && i + 1 < my_count)
+            if (N_DEEP == 1 && i + 1 < my_count)
                 issue_chunk_warp<HD>(p, my_stages, my_stages + CHUNK * HD, &my_bars[0],
                                      chunk_of(my_first + N_WARPS * (i + 1)) * CHUNK, lo_tile, hi_tile, kept, bt, kbase,
                                      vbase, page_stride, lane, cached_for(i + 1));
@@ -798,9 +800,9 @@ attention_mma_kernel(const MmaAttnParams p) {
 template <int HD, bool NARROW, bool BIASED, Keys KEYS>
 int launch_mma_kernel(const MmaAttnParams& p, cudaStream_t stream) {
     const size_t stage_bytes = 2 * (size_t)CHUNK * HD * sizeof(__nv_bfloat16);
-    constexpr int n_warps = NARROW && KEYS == ALL_KEYS ? NARROW_WARPS : OWN_WARPS;
+    constexpr int n_warps = KEYS == ALL_KEYS ? NARROW_WARPS : OWN_WARPS, n_deep = KEYS == ALL_KEYS ? NARROW_STAGES : OWN_STAGES;
     const dim3 block(NARROW ? 32 * n_warps : MMA_THREADS);
-    size_t smem = stage_bytes * (NARROW ? NARROW_STAGES * n_warps : WIDE_STAGES);
+    size_t smem = stage_bytes * (NARROW ? n_deep * n_warps : WIDE_STAGES);
     if (NARROW) {
         const size_t reduce = (size_t)n_warps * 16 * (HD + 8 + 2) * sizeof(float);
         if (reduce > smem) smem = reduce;

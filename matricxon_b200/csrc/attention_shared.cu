@@ -386,6 +386,24 @@ int best_parts(long long blocks, int chunks, int room, int start, int uneven) {
     return best;
 }
 
+// Parts of the shared keys on tcgen05, a block an SM. The own keys' blocks, which are bound by memory, find no room beside one of
+// these, so the parts also say how many SMs are left to them while these run: the two should end together. Of 128 requests on
+// 32,768 shared keys and up to 2,048 own ones (32 tiles of heads) 1, 2, 3, 4 and 8 parts took 320, 164, 182, 189 and 199 us; of 32
+// on 2,048 and 3,000 under a window (12) 2, 4, 8 and 11 took 37, 40, 44 and 45. As measured there, a tile of 128 keys takes 1.15 us,
+// a block's start and end four of them, an SM takes 2.7 chunks of 32 own keys a us and the memory 330.
+int balanced_parts(long long blocks, int chunks, int n_sm, double own_work, double join_us) {
+    int best = 1;
+    double least = 0.0;
+    for (int parts = 1; parts <= 32 && parts <= chunks; ++parts) {
+        const long long rounds = (blocks * parts + n_sm - 1) / n_sm;
+        const double busy = 1.15 * rounds * ((chunks + parts - 1) / parts + 4), left = rounds == 1 ? (double)(n_sm - blocks * parts) : 0.0;
+        const double memory = 330.0 * n_sm / 148.0, beside = busy * (2.7 * left < memory ? 2.7 * left : memory);
+        const double time = busy + (own_work > beside ? (own_work - beside) / memory : 0.0) + join_us * parts;
+        if (parts == 1 || time < least) { best = parts; least = time; }
+    }
+    return best;
+}
+
 SharedPlan make_plan(int dtype, int head_dim, int page_size, bool aligned, int n_tokens, int n_heads, int n_kv_heads, int n_seqs,
                      int n_groups, int max_q_len, int max_shared_len, int max_own_len, int n_sm) {
     SharedPlan plan;
@@ -399,13 +417,18 @@ SharedPlan make_plan(int dtype, int head_dim, int page_size, bool aligned, int n
     const int shared_rows = tc ? 128 / group * group : (mma ? 64 : SH_ROWS);
     plan.shared_tiles = (int)min(rows / shared_rows + n_groups, rows);
     plan.own_tiles = mma ? (plan.narrow ? n_seqs : (int)min(rows / 64 + n_seqs, rows)) : n_tokens * ((group + SH_ROWS - 1) / SH_ROWS);
-    // Parts: blocks run in rounds of as many as fit the GPU (tcgen05 one an SM, narrow tiles two, the others three), and a round
+    // Parts: blocks run in rounds of as many as fit the GPU (narrow tiles two an SM, the others but tcgen05 three), and a round
     // takes as long as a block's chunks and its start. The number of parts with the shortest rounds is taken; the tiles of a
     // group each end in the middle of one, so there may be a tile a group more.
     const int shared_chunks = (max(max_shared_len, 1) + (tc ? 127 : 31)) / (tc ? 128 : 32), own_chunks = max(max_own_len, 1) / 32 + 1;
     const long long shared_blocks = (rows + shared_rows - 1) / shared_rows * n_kv_heads, own_blocks = (long long)plan.own_tiles * n_kv_heads;
-    plan.shared_parts = max_shared_len <= 0 ? 0 : best_parts(shared_blocks, shared_chunks, tc ? n_sm : 3 * n_sm, tc ? 4 : 8, 0);
-    plan.own_parts = best_parts(own_blocks, (own_chunks + 3) / 4, plan.narrow ? 2 * n_sm : 3 * n_sm, 3, 1);
+    const int own_unit = plan.narrow ? 3 : (mma ? 2 : 1);       // chunks that a block takes at a time
+    plan.own_parts = best_parts(own_blocks, (own_chunks + own_unit - 1) / own_unit, plan.narrow ? 2 * n_sm : 3 * n_sm, 3, 1);
+    // the join reads and writes a part's values, float, at some 5 TB/s; own lengths are taken to be half the longest
+    const double join_us = (double)n_tokens * n_heads * head_dim * 8.0 / 5e6, own_work = (double)own_blocks * own_chunks / 2.0;
+    plan.shared_parts = max_shared_len <= 0 ? 0
+                        : tc ? balanced_parts(shared_blocks, shared_chunks, n_sm, own_work, join_us)
+                             : best_parts(shared_blocks, shared_chunks, 3 * n_sm, 8, 0);
     return plan;
 }
 
