@@ -132,40 +132,55 @@ shared_simt_kernel(const SharedAttnParams p) {
     const int* bt = p.block_tables + (size_t)seq * p.bt_stride;
     const T* cache = reinterpret_cast<const T*>(p.cache);
     const size_t head_stride = (size_t)p.page_size * hd;
-    auto page_of = [&](int key) -> long long {
-        const int lp = key / p.page_size;
-        const long long page = lp < p.bt_stride ? bt[lp] : -1;
-        return page >= 0 && page < p.n_pages ? page : -1;
-    };
     auto bring = [&](int c) {
         uint4* k_s = stages + (size_t)(c & 1) * stage_pieces;
         uint4* v_s = k_s + SH_KEYS * cpr;
         const int c0 = (first_chunk + c) * SH_KEYS;
-        // a warp a key
-#pragma unroll 4
-        for (int j = warp; j < SH_KEYS; j += SH_WARPS) {
-            const int key = c0 + j;
-            const bool seen = key >= lo && key <= hi;
-            const long long page = seen ? page_of(key) : -1;
-            if (seen && page < 0 && lane == 0) atomicOr(p.status, MX_STATUS_BAD_PAGE);
-            const T* from = cache + ((size_t)max(page, 0LL) * 2 * p.n_kv_heads + kh) * head_stride + (size_t)(key % p.page_size) * hd;
-            for (int piece = lane; piece < cpr; piece += 32)
-                copy16(&k_s[j * cpr + (piece ^ (j & swz_mask))], page >= 0 ? from + (size_t)piece * E : cache, page >= 0);
+        // a lane looks up a key's page, for the whole warp; a run of E keys lies inside a page
+        const int key = c0 + lane, lp = key / p.page_size, offset = key - lp * p.page_size, run0 = key - key % E;
+        int page = -1;
+        if (run0 <= hi && run0 + E - 1 >= lo) {
+            if (lp < p.bt_stride) page = bt[lp];
+            if (page < 0 || page >= p.n_pages) {
+                page = -1;
+                if (key >= lo && key <= hi) atomicOr(p.status, MX_STATUS_BAD_PAGE);
+            }
         }
-        // a run of E keys lies inside a page: a thread keeps to one run and walks the dimensions
-        const int run = tid % RUNS, key0 = c0 + run * E;
-        const long long page = key0 <= hi && key0 + E - 1 >= lo ? page_of(key0) : -1;
-        const T* from = cache + ((size_t)max(page, 0LL) * 2 * p.n_kv_heads + p.n_kv_heads + kh) * head_stride + key0 % p.page_size;
+        // a warp a key
+#pragma unroll
+        for (int i = 0; i < SH_KEYS / SH_WARPS; ++i) {
+            const int j = warp + i * SH_WARPS, pg = __shfl_sync(0xffffffffu, page, j), off = __shfl_sync(0xffffffffu, offset, j);
+            const bool there = pg >= 0 && c0 + j >= lo && c0 + j <= hi;
+            const T* from = cache + ((size_t)max(pg, 0) * 2 * p.n_kv_heads + kh) * head_stride + (size_t)off * hd;
+            for (int piece = lane; piece < cpr; piece += 32)
+                copy16(&k_s[j * cpr + (piece ^ (j & swz_mask))], there ? from + (size_t)piece * E : cache, there);
+        }
+        // a thread keeps to one run of keys and walks the dimensions
+        const int run = tid % RUNS, pg = __shfl_sync(0xffffffffu, page, run * E), off = __shfl_sync(0xffffffffu, offset, run * E);
+        const T* from = cache + ((size_t)max(pg, 0) * 2 * p.n_kv_heads + p.n_kv_heads + kh) * head_stride + off;
 #pragma unroll 4
         for (int d = tid / RUNS; d < hd; d += SH_THREADS / RUNS)
-            copy16(&v_s[d * RUNS + (run ^ (d & (RUNS - 1)))], page >= 0 ? from + (size_t)d * p.page_size : cache, page >= 0);
+            copy16(&v_s[d * RUNS + (run ^ (d & (RUNS - 1)))], pg >= 0 ? from + (size_t)d * p.page_size : cache, pg >= 0);
     };
+    // the queries and the first keys set out together
+    float query[SH_ROWS_PER_WARP][8];
+#pragma unroll
+    for (int i = 0; i < SH_ROWS_PER_WARP; ++i) {
+        const int r = warp + i * SH_WARPS;
+        const T* from = reinterpret_cast<const T*>(p.q) + (r < rows ? (size_t)row_token[r] * p.q_stride + (size_t)row_head[r] * hd : 0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) query[i][j] = r < rows && lane + 32 * j < hd ? to_float(from[lane + 32 * j]) : 0.f;
+    }
     if (c_begin < c_end) bring(c_begin);
     asm volatile("cp.async.commit_group;\n" ::: "memory");
 
-    for (int r = warp; r < rows; r += SH_WARPS)
-        for (int d = lane; d < hd; d += 32)
-            q_s[r * hd + d] = to_float(reinterpret_cast<const T*>(p.q)[(size_t)row_token[r] * p.q_stride + (size_t)row_head[r] * hd + d]);
+#pragma unroll
+    for (int i = 0; i < SH_ROWS_PER_WARP; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (warp + i * SH_WARPS < rows && lane + 32 * j < hd) q_s[(warp + i * SH_WARPS) * hd + lane + 32 * j] = query[i][j];
+    for (int i = rows * SH_KEYS + tid; i < SH_ROWS * SH_KEYS; i += SH_THREADS) p_s[i] = 0.f;
+    if (tid < SH_ROWS) row_alpha[tid] = 1.f;
     float acc[SH_ROWS][SLOTS];
 #pragma unroll
     for (int r = 0; r < SH_ROWS; ++r)
@@ -186,6 +201,7 @@ shared_simt_kernel(const SharedAttnParams p) {
         float s[SH_ROWS_PER_WARP];
 #pragma unroll
         for (int i = 0; i < SH_ROWS_PER_WARP; ++i) s[i] = 0.f;
+#pragma unroll 4
         for (int piece = 0; piece < cpr; ++piece) {
             float kf[E];
             unpack16<T>(k_s[lane * cpr + (piece ^ (lane & swz_mask))], kf);
@@ -239,15 +255,16 @@ shared_simt_kernel(const SharedAttnParams p) {
             const int d = tid + slot * SH_THREADS;
             if (d < hd) {
 #pragma unroll
-                for (int r = 0; r < SH_ROWS; ++r)
-                    if (r < rows) acc[r][slot] *= row_alpha[r];
+                for (int r = 0; r < SH_ROWS; ++r) acc[r][slot] *= row_alpha[r];
 #pragma unroll 2
                 for (int run = 0; run < RUNS; ++run) {
                     float v[E];
                     unpack16<T>(v_s[d * RUNS + (run ^ (d & (RUNS - 1)))], v);
 #pragma unroll
-                    for (int r = 0; r < SH_ROWS; ++r)
-                        if (r < rows) {
+                    for (int r0 = 0; r0 < SH_ROWS; r0 += 4) {
+                        if (r0 >= rows) break;               // rows of a started four that are none have weights of zero
+#pragma unroll
+                        for (int r = r0; r < r0 + 4; ++r) {
                             const float4* pp = reinterpret_cast<const float4*>(p_s + r * SH_KEYS + run * E);
 #pragma unroll
                             for (int e4 = 0; e4 < E / 4; ++e4) {
@@ -256,6 +273,7 @@ shared_simt_kernel(const SharedAttnParams p) {
                                                fmaf(w.y, v[4 * e4 + 1], fmaf(w.x, v[4 * e4], acc[r][slot]))));
                             }
                         }
+                    }
                 }
             }
         }
