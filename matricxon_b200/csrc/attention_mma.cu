@@ -259,7 +259,8 @@ attention_mma_kernel(const MmaAttnParams p) {
     __shared__ __align__(8) unsigned long long bars[N_STAGES];
     __shared__ int narrow_table[NARROW ? NARROW_TABLE : 1];   // the sequence's first block-table entries
 
-    if (KEYS == SHARED_KEYS) pdl_wait();
+    // the shared keys' kernel waits for all that the two read, lengths and tables among it (a kernel may have laid them out)
+    if (KEYS == SHARED_KEYS || (KEYS == OWN_KEYS && !p.shared.beside)) pdl_wait();
     if (!p.beside) pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
@@ -271,7 +272,7 @@ attention_mma_kernel(const MmaAttnParams p) {
         if (found.tokens <= 0) return;
         seq = found.seq; tile_row0 = found.first; q_start = found.q_start; q_len = found.tokens;
     } else if (KEYS == OWN_KEYS && !NARROW) {
-        const SequenceTile found = find_sequence_tile(p.cu_q, p.shared.n_seqs, tile, TILE_ROWS, p.group, lane);
+        const SequenceTile found = find_sequence_tile(p.shared, p.cu_q, tile, TILE_ROWS, p.group, lane);
         if (found.seq < 0) {
             wait_for_shared_keys();
             return;
@@ -290,7 +291,7 @@ attention_mma_kernel(const MmaAttnParams p) {
     const int group = p.group;
     if (KEYS != SHARED_KEYS) {
         q_start = p.cu_q[seq];
-        q_len = p.cu_q[seq + 1] - q_start;
+        q_len = (KEYS == OWN_KEYS ? min(p.cu_q[seq + 1], p.shared.n_tokens) : p.cu_q[seq + 1]) - q_start;
         ctx = p.context_lens[seq];
     }
     const int own_from = KEYS == OWN_KEYS && p.shared.lens != nullptr ? p.shared.lens[seq] : 0;
@@ -406,7 +407,7 @@ attention_mma_kernel(const MmaAttnParams p) {
         issue_chunk_warp<HD>(p, my_stages, my_stages + CHUNK * HD, &my_bars[0], chunk_of(my_first) * CHUNK, lo_tile,
                              hi_tile, kept, bt, kbase, vbase, page_stride, lane, cached_for(0));
     // queries and the newest keys and values come from the kernels before this one
-    if (KEYS == ALL_KEYS || (KEYS == OWN_KEYS && !p.shared.beside)) pdl_wait();
+    if (KEYS == ALL_KEYS) pdl_wait();
     if (p.beside) pdl_trigger();                        // what was waited for is now there for the next kernel too
     // Q fragments: 16 bytes of each owned row per 32-wide block. A row beyond the tile reads the
     // tile's last row (r_tok, r_head point there): its scores are masked and it is never written, and

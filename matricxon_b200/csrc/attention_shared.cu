@@ -304,7 +304,7 @@ constexpr int JOIN_WARPS = 4;
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
 shared_join_kernel(const float* part_o, const float* part_ml, T* out, int out_stride, const int* cu_q, const float* sink,
-                   int n_heads, int head_dim, long long n_pairs, const SharedPrefixParams shared) {
+                   int n_heads, int head_dim, long long n_pairs, const SharedPrefixParams shared, int* status) {
     pdl_trigger();
     const long long pair = (long long)blockIdx.x * JOIN_WARPS + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
@@ -313,7 +313,9 @@ shared_join_kernel(const float* part_o, const float* part_ml, T* out, int out_st
     part_o = after_wait(part_o);
     part_ml = after_wait(part_ml);
     const int token = (int)(pair / n_heads), head = (int)(pair - (long long)token * n_heads);
-    if (token >= cu_q[shared.n_seqs]) return;
+    const int rows = cu_q[shared.n_seqs];
+    if (rows > shared.n_tokens && pair == 0 && lane == 0) atomicOr(status, MX_STATUS_BAD_STEP);
+    if (token >= rows) return;
     const size_t base = (size_t)pair * shared.n_parts;
     float m = -INFINITY;
     for (int s = lane; s < shared.n_parts; s += 32) m = fmaxf(m, part_ml[(base + s) * 2]);
@@ -374,7 +376,7 @@ int launch_join(const SharedAttnParams& p, T* out, int out_stride, const float* 
     const long long pairs = (long long)p.n_tokens * p.n_heads;
     const cudaError_t e = mx_launch_beside(shared_join_kernel<T>, dim3((unsigned)((pairs + JOIN_WARPS - 1) / JOIN_WARPS)),
                                            dim3(JOIN_WARPS * 32), 0, stream, (const float*)p.part_o, (const float*)p.part_ml, out, out_stride,
-                                           p.cu_q, sink, p.n_heads, p.head_dim, pairs, p.shared);
+                                           p.cu_q, sink, p.n_heads, p.head_dim, pairs, p.shared, p.status);
     if (e != cudaSuccess) {
         mx_set_error("attention over shared keys: launch failed: %s", cudaGetErrorString(e));
         return (int)e;
@@ -507,7 +509,7 @@ extern "C" int mx_paged_attention_shared(const void* q, int dtype, int q_stride,
     p.group = n_heads / n_kv_heads; p.head_dim = head_dim; p.page_size = page_size; p.window = window; p.scale = scale;
     p.softcap = softcap;
     p.shared.first = first; p.shared.lens = lens; p.shared.tok_seq = tok_seq; p.shared.positions = positions;
-    p.shared.n_groups = n_groups; p.shared.n_seqs = n_seqs; p.shared.n_shared_parts = plan.shared_parts;
+    p.shared.n_groups = n_groups; p.shared.n_seqs = n_seqs; p.shared.n_tokens = n_tokens; p.shared.n_shared_parts = plan.shared_parts;
     p.shared.n_parts = plan.shared_parts + plan.own_parts;
     p.shared.beside = 0;
     if (plan.shared_parts == 0) p.shared.lens = nullptr;

@@ -14,6 +14,7 @@ struct SharedPrefixParams {
     const int* positions;    // [tokens]
     int n_groups;
     int n_seqs;
+    int n_tokens;            // rows that there are: sequences that bring more are cut off there (and reported by the join)
     int n_parts;             // parts of a token and head's softmax, those of the shared keys first
     int n_shared_parts;
     int beside;              // the kernel of the shared keys was launched just before this one, which begins beside it
@@ -71,8 +72,8 @@ __device__ __forceinline__ GroupTile find_group_tile(const SharedPrefixParams& p
         int seq = 0, start = 0, tokens = 0;
         if (g < p.n_groups) {
             seq = min(max(p.first[g], 0), p.n_seqs);
-            start = cu_q[seq];
-            tokens = cu_q[min(max(p.first[g + 1], 0), p.n_seqs)] - start;
+            start = min(cu_q[seq], p.n_tokens);
+            tokens = min(cu_q[min(max(p.first[g + 1], 0), p.n_seqs)], p.n_tokens) - start;
         }
         const int tiles = tokens > 0 ? (tokens * rows + per_tile - 1) / per_tile : 0;
         int through = tiles;
@@ -99,11 +100,11 @@ __device__ __forceinline__ GroupTile find_group_tile(const SharedPrefixParams& p
 struct SequenceTile {
     int seq, row;            // seq < 0: there is no such tile
 };
-__device__ __forceinline__ SequenceTile find_sequence_tile(const int* cu_q, int n_seqs, int tile, int rows, int group, int lane) {
+__device__ __forceinline__ SequenceTile find_sequence_tile(const SharedPrefixParams& p, const int* cu_q, int tile, int rows, int group, int lane) {
     int before = 0;
-    for (int s0 = 0; s0 < n_seqs; s0 += 32) {
+    for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
         const int s = s0 + lane;
-        const int mine = s < n_seqs ? (cu_q[s + 1] - cu_q[s]) * group : 0;
+        const int mine = s < p.n_seqs ? max(0, min(cu_q[s + 1], p.n_tokens) - cu_q[s]) * group : 0;
         const int tiles = (mine + rows - 1) / rows;
         int through = tiles;
 #pragma unroll

@@ -716,7 +716,7 @@ def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, 
     sequence s brings rows ``cu_q[s] .. cu_q[s + 1] - 1``, row i of it at position ``context_lens[s] + i``, which
     ``positions`` and ``tok_seq`` repeat row by row. Rows from ``cu_q[-1]`` on are left alone.
 
-    ``max_q_len``: no sequence brings more tokens (one that does sets the status word). ``max_shared_len``,
+    ``max_q_len``: no sequence brings more tokens, and all together at most ``n_tokens`` (otherwise the status word is set). ``max_shared_len``,
     ``max_own_len`` (keys that a sequence shares, and does not) are for sizing: with other numbers the result is the same
     up to rounding. All three are host numbers, so that a captured step can be replayed with other lengths and groups
     below them. ``scratch`` (float32) is taken from torch's allocator where none is given. The keys and values that any
@@ -794,6 +794,8 @@ def step_tables(q_lens: torch.Tensor, context_lens: torch.Tensor, rows: torch.Te
               ("tok_seq", tok_seq, per_token), ("cu_q", cu_q, (n_seqs + 1,)), ("slots", slots, per_token),
               ("block_tables", block_tables, (n_seqs, width)), ("taken", taken, None), ("status", status, None),
               ("shared_rows", shared_rows, per_seq), ("shared_pages", shared_pages, per_seq))
+    if block_tables.data_ptr() == tables.data_ptr():
+        raise KernelLibraryError("block_tables are the step's own: tables hold what the requests keep")
     if n_free.numel() < 1 or taken.numel() < 1 or status.numel() < 1:
         raise KernelLibraryError("n_free, taken and status hold a number each")
     if rows is None and tables.shape[0] < n_seqs:
@@ -826,8 +828,8 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, token_offsets: torch.
     or multiplied (negative) by ``repeat_penalty[r]`` and then loses ``frequency_penalty[r] * c + presence_penalty[r]``
     (float32 [rows]). ``bias_values`` (float32) are added at ``bias_ids``, row r's at ``bias_offsets[r]:bias_offsets[r + 1]``; of
     two of one token the later one counts. ``mask_words`` (int32 [masks, words]): bit v % 32 of word v / 32 says whether
-    token v may be taken; a score that may not becomes -infinity. Row r goes by mask ``mask_rows[r]`` (-1: none), or by
-    mask r where there is no ``mask_rows``. Ids outside the vocabulary are passed over. Rows of ``logits`` and ``out`` may be
+    token v may be taken; a score that may not becomes -infinity. Row r goes by mask ``mask_rows[r]`` (a number that names no
+    mask, as -1: none), or by mask r where there is no ``mask_rows``. Ids outside the vocabulary are passed over. Rows of ``logits`` and ``out`` may be
     strided."""
     here, code = _here("logits", logits), dtype_code(logits.dtype)
     if out.dtype is not torch.float32 or out.get_device() != here:

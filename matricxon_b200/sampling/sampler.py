@@ -46,6 +46,7 @@ class RequestSampler:
         self._distinct: set[int] = set()
         self._distinct_list: list[int] = []
         self._mask_words: np.ndarray | None = None
+        self.adjusts = config.adjusts_scores          # asked for every row of every step
 
     def next_uniform(self, ahead: int = 0) -> float:
         """The uniform of the next token, or of the one ``ahead`` tokens after it."""
@@ -59,7 +60,7 @@ class RequestSampler:
 
     def penalty_ids(self) -> list[int]:
         """The generated ids that the sampling kernel penalises: none where their scores were adjusted before it."""
-        if self.config.repeat_penalty == 1.0 or self.config.adjusts_scores:
+        if self.config.repeat_penalty == 1.0 or self.adjusts:
             return []
         return self._distinct_list
 
@@ -124,7 +125,7 @@ class BatchSampler:
             offsets.append(len(ids))
         total = 4 * n + n + (n + 1) + len(ids)
         # rows whose scores are adjusted first (adjust_logits) bring what that takes behind the rest of the buffer
-        adjusting = [s.config.adjusts_scores for s in samplers]
+        adjusting = [s.adjusts for s in samplers]
         extra, places = self._adjustments(samplers, total) if any(adjusting) else (None, None)
         plain = total
         if extra is not None:
@@ -189,7 +190,7 @@ class BatchSampler:
         repeat, presence, frequency = [], [], []
         for sampler in samplers:
             config = sampler.config
-            adjusts = config.adjusts_scores
+            adjusts = sampler.adjusts
             if adjusts and (config.repeat_penalty != 1.0 or config.presence_penalty or config.frequency_penalty):
                 tokens.extend(sampler.generated)
             token_offsets.append(len(tokens))

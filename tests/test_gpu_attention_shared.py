@@ -311,6 +311,22 @@ def test_a_request_with_more_tokens_than_said_is_reported():
     assert step.d["status"].item() == 16
 
 
+def test_sequences_beyond_the_rows_are_cut_off_and_reported():
+    """Sequences that together bring more tokens than there are rows: the rows that there are come out as ever, nothing is
+    written behind them."""
+    for shape in (SHAPES[0], SHAPES[5], SHAPES[10]):
+        step = Step([(64, [(30, 3), (9, 4)])], *shape, seed=3)
+        out = step.run().clone()
+        step.d["status"].zero_()
+        rows, step.n = step.n, 5
+        scratch = torch.full((1 << 22,), 7.0, device=DEV)
+        short = step.run(out=torch.full((rows, step.heads * step.dim), float("nan"), dtype=step.dtype, device=DEV), scratch=scratch)
+        assert step.d["status"].item() == 16
+        assert torch.isnan(short[5:]).all() and (short[:5].float() - out[:5].float()).abs().max() <= 4 * 2 ** -8 * 5.0
+        used = (5 * step.heads * 32 * 2) * (step.dim + 2)            # at most 32 parts of either kind
+        assert (scratch[used:] == 7).all()
+
+
 def test_refusals():
     from matricxon_b200.ops import kernels
     from matricxon_b200.ops.library import KernelLibraryError

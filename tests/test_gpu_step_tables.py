@@ -271,6 +271,10 @@ def test_refusals():
     broken(block_tables=lambda t: t[:, :-1].contiguous())
     broken(shared_rows=ints([-1, -1]))
     broken(keep_first=-1)
+    case = Case([1, 2], [5, 6], 16, use_rows=False).device()      # the step's tables in place of the requests'
+    case.inputs["tables"] = case.outputs["block_tables"]
+    with pytest.raises(KernelLibraryError):
+        case.run()
     case = Case([1, 2], [5, 6], 16).device()
     case.page = 0
     with pytest.raises(KernelLibraryError):
