@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(DEAL_THREADS) deal_ids_kernel(const AdjustPara
     pdl_trigger();                                    // the scores' kernel begins beside this one
     const int first = p.token_offsets ? p.token_offsets[row] : 0, last = p.token_offsets ? p.token_offsets[row + 1] : 0;
     const int pending = p.pending ? p.pending[row] : -1, shift = shift_of(p, row);
-    const int n = max(last - first, 0) + 1;
+    const int n = max(last - first, 0) + 1, log_stretch = 31 - __clz(p.stretch);       // a power of two
     // the stretches of ids k0 + tid, + DEAL_THREADS, ... (-1: none)
     auto ahead = [&](int k0, int* id, int* to) {
 #pragma unroll
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(DEAL_THREADS) deal_ids_kernel(const AdjustPara
             id[e] = k >= n ? -1 : (k == n - 1 ? pending : p.token_ids[first + k]);
         }
 #pragma unroll
-        for (int e = 0; e < AL_AHEAD; ++e) to[e] = id[e] >= 0 && id[e] < p.vocab ? (id[e] + shift) / p.stretch : -1;
+        for (int e = 0; e < AL_AHEAD; ++e) to[e] = id[e] >= 0 && id[e] < p.vocab ? (id[e] + shift) >> log_stretch : -1;
     };
     int id[AL_AHEAD], to[AL_AHEAD];
     for (int i = tid; i < n_blocks; i += DEAL_THREADS) count[i] = 0;
@@ -114,18 +114,11 @@ __global__ void __launch_bounds__(DEAL_THREADS) deal_ids_kernel(const AdjustPara
     }
     __syncthreads();
     int* dealt = p.dealt + (size_t)first + row;       // behind the lists before this one, and a pending id each
-    for (int k0 = 0; k0 < n; k0 += AL_AHEAD * DEAL_THREADS) {    // the same trips for every lane
+    for (int k0 = 0; k0 < n; k0 += AL_AHEAD * DEAL_THREADS) {
         ahead(k0, id, to);
 #pragma unroll
-        for (int e = 0; e < AL_AHEAD; ++e) {
-            // most ids are frequent tokens, of one stretch: its lanes take their places together
-            const unsigned peers = __match_any_sync(0xffffffffu, to[e]);
-            const int leader = __ffs(peers) - 1;
-            int at = 0;
-            if (to[e] >= 0 && lane == leader) at = atomicAdd(&count[to[e]], __popc(peers));
-            at = __shfl_sync(0xffffffffu, at, leader) + __popc(peers & ((1u << lane) - 1u));
-            if (to[e] >= 0) dealt[at] = id[e];
-        }
+        for (int e = 0; e < AL_AHEAD; ++e)
+            if (to[e] >= 0) dealt[atomicAdd(&count[to[e]], 1)] = id[e];
     }
 }
 
@@ -294,7 +287,7 @@ __global__ void __launch_bounds__(AL_THREADS, 5) adjust_logits_kernel(const Adju
     }
 }
 
-// Scores of a block: a turn while that makes no more than some eight blocks an SM, else four turns (32 KB of counts).
+// Scores of a block, a power of two: a turn while that makes no more than some eight blocks an SM, else four turns (32 KB of counts).
 int stretch_of(int n_rows, int vocab) { return (long long)n_rows * vocab <= 8LL * 148 * AL_TURN ? AL_TURN : 4 * AL_TURN; }
 
 long long blocks_of(int n_rows, int vocab) { return ((long long)vocab + 3 + stretch_of(n_rows, vocab) - 1) / stretch_of(n_rows, vocab); }

@@ -27,6 +27,8 @@
 //     (each warp's weight per row computed once, then float4 sums). A warp's first chunk, if
 //     all its keys were cached by earlier steps, is asked for before the kernel waits for its
 //     predecessor in the stream (the one that computes the queries and this step's keys).
+// For sequences that have their first keys in common (attention_shared.cu) the same tiles walk one part of the keys each: wide
+// ones of a group's rows the shared keys, narrow (three warps a block) or wide ones each sequence's own.
 // Every wait on an mbarrier is bounded: after SPIN_LIMIT polls the kernel sets
 // MX_STATUS_WAIT_TIMEOUT in the step's status word and goes on, so it always ends.
 // Per chunk and warp: S = Q K^T with mma.sync.m16n8k16 (bf16 in, float out), float online
@@ -48,14 +50,15 @@ constexpr int MMA_WARPS = 4;        // wide tiles: 16 rows each
 constexpr int MMA_THREADS = MMA_WARPS * 32;
 constexpr int NARROW_WARPS = 8;     // narrow tiles: all warps hold the same rows and share the chunks
 constexpr int NARROW_THREADS = NARROW_WARPS * 32;
-constexpr int OWN_WARPS = 3;        // the same for OWN_KEYS: fewer warps, each with a chunk on its way while it works on another,
-constexpr int OWN_STAGES = 2;       // and two blocks an SM, so that one begins and ends while the other reads
+// Narrow tiles of OWN_KEYS: fewer warps, each with a chunk on its way while it works on another, and two blocks an SM, so that
+// one begins and ends while the other reads (128 requests with 530 MB of own keys, us: eight warps of one chunk 134, two blocks
+// of four 120, two of three with two chunks 103, which is 5.9 TB/s).
+constexpr int OWN_WARPS = 3, OWN_STAGES = 2, OWN_BLOCKS = 2;
 constexpr int CHUNK = 32;
 constexpr int WIDE_STAGES = 4;      // chunks in flight per block (two pairs), wide tiles
 constexpr int NARROW_STAGES = 1;    // chunks in flight per warp, narrow tiles
 constexpr int NARROW_TABLE = 512;   // block-table entries a narrow tile's block reads ahead (8,192 positions in pages of 16)
 constexpr int SPIN_LIMIT = 1 << 22;
-constexpr int OWN_BLOCKS = 2;       // ... of which an SM holds this many
 
 struct MmaAttnParams {
     const __nv_bfloat16* q;      // [tokens][q_stride], head h at h * HD
@@ -257,10 +260,11 @@ attention_mma_kernel(const MmaAttnParams p) {
     extern __shared__ __align__(128) unsigned char smem_raw[];
     __nv_bfloat16* stages = reinterpret_cast<__nv_bfloat16*>(smem_raw);
     __shared__ __align__(8) unsigned long long bars[N_STAGES];
-    __shared__ int narrow_table[NARROW || KEYS != ALL_KEYS ? NARROW_TABLE : 1];   // the sequence's first block-table entries
+    __shared__ int narrow_table[NARROW || KEYS != ALL_KEYS ? NARROW_TABLE : 1];   // block-table entries: the sequence's first (ALL_KEYS) or the block's
 
     // the shared keys' kernel waits for all that the two read, lengths and tables among it (a kernel may have laid them out)
     if (KEYS == SHARED_KEYS || (KEYS == OWN_KEYS && !p.shared.beside)) pdl_wait();
+    if (KEYS == OWN_KEYS) asm volatile("fence.proxy.async.global;\n" ::: "memory");   // what the copies read, kernels before wrote
     if (!p.beside) pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
