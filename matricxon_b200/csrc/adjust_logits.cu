@@ -18,8 +18,9 @@
 // place in the list among a token's biases says which one holds. What a phase reads it asks for eight at a time.
 // Where a row has many blocks and a long list, a kernel beside deals the ids out to the stretches first, so that each is looked
 // at once, not by every block of the row.
-// 256 rows of 131,071 scores, a third of them allowed, with 6,144 ids each: 90 us, 121 with every block reading the whole list (a copy of
-// such scores takes 47).
+// 256 rows of 131,071 scores, a third of them allowed, with 6,144 ids each: 90 us (a copy of the scores takes 47), 121 with every
+// block reading the whole list, 92 with a kernel after this one that gathers each row's list in a hash table. What is left
+// above the copy are the atomics: shared memory takes some 0.75 lanes of them a cycle and SM, whatever words they go to.
 #include <math.h>
 
 #include "common.cuh"

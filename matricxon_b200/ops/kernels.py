@@ -680,18 +680,16 @@ def _here(name: str, tensor: torch.Tensor) -> int:
     return here
 
 
-def _need_all(here: int, dtype: torch.dtype, *wanted: tuple[str, torch.Tensor | None, tuple | None]) -> None:
-    """Every (name, tensor, shape) of ``wanted`` that has a tensor: contiguous, of ``dtype``, on device ``here`` and of that
-    shape (None: any). One pass of cheap comparisons: an operator of a few microseconds takes up to fifteen tensors."""
-    for name, tensor, shape in wanted:
-        if tensor is None:
-            continue
-        if tensor.dtype is not dtype or tensor.get_device() != here or not tensor.is_contiguous() or (
-                shape is not None and tensor.shape != shape):
+def _need_all(here: int, dtype: torch.dtype, *wanted: tuple[str, torch.Tensor | None, int]) -> None:
+    """Every (name, tensor, numbers) of ``wanted`` that has a tensor: contiguous, of ``dtype``, on device ``here`` and of so many
+    numbers (-1: any). One pass of cheap comparisons: an operator of a few microseconds takes up to fifteen tensors."""
+    for name, tensor, numbers in wanted:
+        if tensor is not None and (tensor.dtype is not dtype or tensor.get_device() != here or not tensor.is_contiguous()
+                                   or (tensor.numel() != numbers and numbers >= 0)):
             _need(tensor, name, dtype)
             if tensor.get_device() != here:
                 raise KernelLibraryError(f"{name} is on {tensor.device}, kernels run on cuda:{here}")
-            raise KernelLibraryError(f"{name} must be {dtype} {list(shape)}, got {list(tensor.shape)}")
+            raise KernelLibraryError(f"{name} must hold {numbers} numbers, got {list(tensor.shape)}")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -722,11 +720,13 @@ def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, 
     below them. ``scratch`` (float32) is taken from torch's allocator where none is given. The keys and values that any
     token of a group sees have to be finite."""
     here, code = _here("q", q), dtype_code(q.dtype)
-    n_seqs, int32 = context_lens.numel(), torch.int32
-    _need_all(here, q.dtype, ("cache", cache, None))
-    _need_all(here, int32, ("context_lens", context_lens, (n_seqs,)), ("block_tables", block_tables, None), ("cu_q", cu_q, (n_seqs + 1,)),
-              ("tok_seq", tok_seq, None), ("positions", positions, None), ("shared_first", shared_first, None),
-              ("shared_lens", shared_lens, (n_seqs,)), ("status", status, None))
+    n_seqs = context_lens.numel()
+    _need_all(here, q.dtype, ("cache", cache, -1))
+    _need_all(here, torch.int32, ("context_lens", context_lens, n_seqs), ("block_tables", block_tables, -1), ("cu_q", cu_q, n_seqs + 1),
+              ("tok_seq", tok_seq, -1), ("positions", positions, -1), ("shared_first", shared_first, -1),
+              ("shared_lens", shared_lens, n_seqs), ("status", status, -1))
+    if sink is not None:
+        _need_all(here, torch.float32, ("sink", sink, n_heads))
     if out.dtype is not q.dtype or out.get_device() != here:
         raise KernelLibraryError(f"out must be {q.dtype} on {q.device}, got {out.dtype} on {out.device}")
     if block_tables.ndim != 2 or block_tables.shape[0] != n_seqs:
@@ -752,15 +752,15 @@ def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, 
     if scratch is None:
         scratch = torch.empty((need + 3) // 4, dtype=torch.float32, device=q.device)
     else:
-        _need_all(here, torch.float32, ("scratch", scratch, None))
+        _need_all(here, torch.float32, ("scratch", scratch, -1))
     if scratch.numel() * 4 < need or scratch.data_ptr() % 16 != 0:
         raise KernelLibraryError(f"attention over shared keys needs {need} bytes of 16-byte aligned scratch")
     check(library().mx_paged_attention_shared(
-        _ptr(q), code, q_stride, _ptr(cache), cache.shape[0], page_size, _ptr(block_tables), block_tables.stride(0),
-        _ptr(cu_q), _ptr(context_lens), _ptr(tok_seq), _ptr(positions), _ptr(shared_first), _ptr(shared_lens), n_seqs,
-        n_groups, n_tokens, n_heads, n_kv_heads, head_dim, int(window or 0), float(scale), float(softcap or 0.0),
-        _sink_ptr(sink, n_heads), _ptr(out), out.stride(0), int(max_q_len), int(max_shared_len), int(max_own_len), n_sm,
-        _ptr(scratch), _ptr(status), _stream()), "paged_attention_shared")
+        q.data_ptr(), code, q_stride, cache.data_ptr(), cache.shape[0], page_size, block_tables.data_ptr(), block_tables.shape[1],
+        cu_q.data_ptr(), context_lens.data_ptr(), tok_seq.data_ptr(), positions.data_ptr(), shared_first.data_ptr(),
+        shared_lens.data_ptr(), n_seqs, n_groups, n_tokens, n_heads, n_kv_heads, head_dim, int(window or 0), float(scale), float(softcap or 0.0),
+        _sink_ptr(sink, n_heads), out.data_ptr(), out.stride(0), int(max_q_len), int(max_shared_len), int(max_own_len), n_sm,
+        scratch.data_ptr(), status.data_ptr(), _stream()), "paged_attention_shared")
     _launched(3 if max_shared_len > 0 else 2)
 
 
@@ -788,12 +788,11 @@ def step_tables(q_lens: torch.Tensor, context_lens: torch.Tensor, rows: torch.Te
     if tables.ndim != 2:
         raise KernelLibraryError(f"tables must be [table rows, width], got {list(tables.shape)}")
     width = tables.shape[1]
-    per_seq, per_token = (n_seqs,), (n_tokens,)
-    _need_all(here, torch.int32, ("q_lens", q_lens, per_seq), ("context_lens", context_lens, per_seq), ("rows", rows, per_seq),
-              ("tables", tables, None), ("free_pages", free_pages, None), ("n_free", n_free, None), ("positions", positions, per_token),
-              ("tok_seq", tok_seq, per_token), ("cu_q", cu_q, (n_seqs + 1,)), ("slots", slots, per_token),
-              ("block_tables", block_tables, (n_seqs, width)), ("taken", taken, None), ("status", status, None),
-              ("shared_rows", shared_rows, per_seq), ("shared_pages", shared_pages, per_seq))
+    _need_all(here, torch.int32, ("q_lens", q_lens, -1), ("context_lens", context_lens, n_seqs), ("rows", rows, n_seqs),
+              ("tables", tables, -1), ("free_pages", free_pages, -1), ("n_free", n_free, -1), ("positions", positions, -1),
+              ("tok_seq", tok_seq, n_tokens), ("cu_q", cu_q, n_seqs + 1), ("slots", slots, n_tokens),
+              ("block_tables", block_tables, n_seqs * width), ("taken", taken, -1), ("status", status, -1),
+              ("shared_rows", shared_rows, n_seqs), ("shared_pages", shared_pages, n_seqs))
     if block_tables.data_ptr() == tables.data_ptr():
         raise KernelLibraryError("block_tables are the step's own: tables hold what the requests keep")
     if n_free.numel() < 1 or taken.numel() < 1 or status.numel() < 1:
@@ -801,10 +800,10 @@ def step_tables(q_lens: torch.Tensor, context_lens: torch.Tensor, rows: torch.Te
     if rows is None and tables.shape[0] < n_seqs:
         raise KernelLibraryError(f"{n_seqs} sequences need as many rows of tables, got {tables.shape[0]}")
     check(library().mx_step_tables(
-        _ptr(q_lens), _ptr(context_lens), _ptr(rows), n_seqs, _ptr(tables), tables.shape[0], width, _ptr(free_pages),
-        free_pages.numel(), _ptr(n_free), int(page_size), int(n_pages), _ptr(shared_rows), _ptr(shared_pages), int(window or 0),
-        int(keep_first), _ptr(positions), _ptr(tok_seq), _ptr(cu_q), _ptr(slots), n_tokens, _ptr(block_tables), _ptr(taken),
-        _ptr(status), _stream()), "step_tables")
+        q_lens.data_ptr(), context_lens.data_ptr(), _ptr(rows), n_seqs, tables.data_ptr(), tables.shape[0], width,
+        free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), int(page_size), int(n_pages), _ptr(shared_rows),
+        _ptr(shared_pages), int(window or 0), int(keep_first), positions.data_ptr(), tok_seq.data_ptr(), cu_q.data_ptr(),
+        slots.data_ptr(), n_tokens, block_tables.data_ptr(), taken.data_ptr(), status.data_ptr(), _stream()), "step_tables")
     _launched()
 
 
@@ -839,12 +838,11 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, token_offsets: torch.
     n_rows, vocab = logits.shape
     if n_rows > 1 and out.stride(0) < vocab:
         raise KernelLibraryError("rows of out must not overlap")
-    per_row, ends = (n_rows,), (n_rows + 1,)
-    _need_all(here, torch.int32, ("token_offsets", token_offsets, ends), ("token_ids", token_ids, None), ("bias_offsets", bias_offsets, ends),
-              ("bias_ids", bias_ids, None), ("mask_words", mask_words, None), ("mask_rows", mask_rows, per_row),
-              ("pending_ids", pending_ids, per_row))
-    _need_all(here, torch.float32, ("repeat_penalty", repeat_penalty, per_row), ("presence_penalty", presence_penalty, per_row),
-              ("frequency_penalty", frequency_penalty, per_row), ("bias_values", bias_values, None))
+    _need_all(here, torch.int32, ("token_offsets", token_offsets, n_rows + 1), ("token_ids", token_ids, -1),
+              ("bias_offsets", bias_offsets, n_rows + 1), ("bias_ids", bias_ids, -1), ("mask_words", mask_words, -1),
+              ("mask_rows", mask_rows, n_rows), ("pending_ids", pending_ids, n_rows))
+    _need_all(here, torch.float32, ("repeat_penalty", repeat_penalty, n_rows), ("presence_penalty", presence_penalty, n_rows),
+              ("frequency_penalty", frequency_penalty, n_rows), ("bias_values", bias_values, -1))
     if mask_words is not None and mask_words.ndim != 2:
         raise KernelLibraryError(f"mask_words must be [masks, words], got {list(mask_words.shape)}")
     if (token_offsets is None) != (token_ids is None):
