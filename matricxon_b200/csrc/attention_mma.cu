@@ -51,8 +51,8 @@ constexpr int MMA_THREADS = MMA_WARPS * 32;
 constexpr int NARROW_WARPS = 8;     // narrow tiles: all warps hold the same rows and share the chunks
 constexpr int NARROW_THREADS = NARROW_WARPS * 32;
 // Narrow tiles of OWN_KEYS: fewer warps, each with a chunk on its way while it works on another, and two blocks an SM, so that
-// one begins and ends while the other reads (128 requests with 530 MB of own keys, us: eight warps of one chunk 134, two blocks
-// of four 120, two of three with two chunks 103, which is 5.9 TB/s).
+// one begins and ends while the other reads (128 requests with 607 MB of own keys: two blocks of four warps with a chunk each
+// 120 us, these 113, which is 5.4 TB/s).
 constexpr int OWN_WARPS = 3, OWN_STAGES = 2, OWN_BLOCKS = 2;
 constexpr int CHUNK = 32;
 constexpr int WIDE_STAGES = 4;      // chunks in flight per block (two pairs), wide tiles
