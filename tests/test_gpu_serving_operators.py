@@ -205,3 +205,41 @@ def test_a_decoding_loop_of_all_three(chained):
             assert float(expected[got[s]]) >= float(expected.max()) - 1e-4 and got[s] % 3 == s % 3
             samplers[s].accept(got[s])
     assert status.item() == 0
+
+
+def test_two_streams_at_once():
+    """Calls of all three queued on two streams, many times over: each gives, bit by bit, what it gives alone."""
+    from test_gpu_adjust_logits import Case as Scores
+    from test_gpu_adjust_logits import adjust
+    from test_gpu_attention_shared import SHAPES, STEPS, Step
+    from test_gpu_step_tables import random_case
+
+    attention = [Step(STEPS["groups"], *SHAPES[0], seed=1), Step(STEPS["portions"], *SHAPES[5], seed=2),
+                 Step([(2048, [(k * 37 % 300, 1) for k in range(20)])], *SHAPES[0], seed=3), Step(STEPS["groups"], *SHAPES[10], seed=4)]
+    scores = [Scores(30, 9001, tokens=400, seed=s) for s in (1, 2)]
+    arguments = [(case.logits.to(DEV), case.device()) for case in scores]
+    tables = [random_case(60, 16, s).device() for s in (3, 4)]
+    expected_tables = [case.expected() for case in tables]
+    alone = [step.run().clone() for step in attention]
+    alone_scores = [adjust(logits, torch.empty_like(logits), **args) for logits, args in arguments]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(25):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got += [(k, attention[k].run()) for k in (i, 2 + i)]
+                got.append((4 + i, adjust(arguments[i][0], torch.empty_like(arguments[i][0]), **arguments[i][1])))
+    torch.cuda.synchronize()
+    for k, out in got:
+        if k < 4:
+            rows = attention[k].cu[-1]
+            assert torch.equal(out[:rows], alone[k][:rows])
+        else:
+            assert torch.equal(out, alone_scores[k - 4])
+    for case, expected in zip(tables, expected_tables):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                assert case.run() == expected
+            torch.cuda.synchronize()
+    assert all(step.d["status"].item() == 0 for step in attention)
