@@ -734,15 +734,16 @@ def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, 
     n_groups = shared_first.numel() - 1
     if n_groups < 1 and n_seqs > 0:
         raise KernelLibraryError("shared_first must hold the start of at least one group and the end of the last")
-    page_size = cache.shape[3] if cache.ndim == 5 else 0
-    if tuple(cache.shape[1:]) != (2, n_kv_heads, page_size, head_dim):
+    n_pages, planes, cached_heads, page_size, cached_dim = cache.shape if cache.ndim == 5 else (0, 0, 0, 0, 0)
+    if planes != 2 or cached_heads != n_kv_heads or cached_dim != head_dim:
         raise KernelLibraryError(f"cache must be [pages, 2, {n_kv_heads}, page size, {head_dim}], got {list(cache.shape)}")
+    width = n_heads * head_dim
     if min(tok_seq.numel(), positions.numel()) < n_tokens or q.ndim != 2 or q.shape[0] < n_tokens:
         raise KernelLibraryError(f"q, tok_seq and positions must hold {n_tokens} rows")
-    if q.stride(1) != 1 or q_stride != q.stride(0) or q.shape[1] < n_heads * head_dim:
-        raise KernelLibraryError(f"q must hold rows of {n_heads * head_dim} numbers, q_stride apart, got {list(q.shape)}")
-    if out.ndim != 2 or out.shape[0] < n_tokens or out.shape[1] != n_heads * head_dim or out.stride(1) != 1:
-        raise KernelLibraryError(f"out must hold {n_tokens} rows of {n_heads * head_dim} numbers, got {list(out.shape)}")
+    if q.stride() != (q_stride, 1) or q.shape[1] < width:
+        raise KernelLibraryError(f"q must hold rows of {width} numbers, q_stride apart, got {list(q.shape)}")
+    if out.ndim != 2 or out.shape[0] < n_tokens or out.shape[1] != width or out.stride(1) != 1:
+        raise KernelLibraryError(f"out must hold {n_tokens} rows of {width} numbers, got {list(out.shape)}")
     if n_tokens <= 0 or n_seqs == 0:
         return
     aligned = q_stride % 8 == 0 and q.data_ptr() % 16 == 0 and cache.data_ptr() % 16 == 0
@@ -756,7 +757,7 @@ def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, 
     if scratch.numel() * 4 < need or scratch.data_ptr() % 16 != 0:
         raise KernelLibraryError(f"attention over shared keys needs {need} bytes of 16-byte aligned scratch")
     check(library().mx_paged_attention_shared(
-        q.data_ptr(), code, q_stride, cache.data_ptr(), cache.shape[0], page_size, block_tables.data_ptr(), block_tables.shape[1],
+        q.data_ptr(), code, q_stride, cache.data_ptr(), n_pages, page_size, block_tables.data_ptr(), block_tables.shape[1],
         cu_q.data_ptr(), context_lens.data_ptr(), tok_seq.data_ptr(), positions.data_ptr(), shared_first.data_ptr(),
         shared_lens.data_ptr(), n_seqs, n_groups, n_tokens, n_heads, n_kv_heads, head_dim, int(window or 0), float(scale), float(softcap or 0.0),
         _sink_ptr(sink, n_heads), out.data_ptr(), out.stride(0), int(max_q_len), int(max_shared_len), int(max_own_len), n_sm,
