@@ -87,7 +87,7 @@ struct MmaAttnParams {
 };
 
 // Which keys a launch covers. OWN_KEYS: those of a sequence from shared.lens[sequence] on; SHARED_KEYS (wide tiles): those
-// below it, for tiles of a group's tokens, read through the group's first sequence (attention_shared.cu). Both write parts.
+// below it, for tiles of a group's tokens, on pages that the group shares (attention_shared.cu). Both write parts.
 enum Keys { ALL_KEYS, OWN_KEYS, SHARED_KEYS };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2,
@@ -199,7 +199,7 @@ __device__ __forceinline__ void issue_chunk(const MmaAttnParams& p, __nv_bfloat1
 }
 
 // The same by one warp for narrow tiles, a lane a page; `cached`: this chunk's block-table entries, read ahead into shared
-// memory (null: from the table). A decode step's attention is a chain of latencies, and one lane
+// memory (null: from the table), `group`: pages that a group's sequences share (null: a sequence's own). A decode step's attention is a chain of latencies, and one lane
 // that walks the pages and issues every copy took as long as the chunk's arithmetic (2,000 cycles; with this and the
 // divisions by the group taken out of a one-token tile's way, one request at 3,100 tokens of the 3B sizes decodes in
 // 1.64 instead of 1.68 ms a step). Merging the key splits as a cluster of blocks, without the kernel that follows, gained
@@ -209,7 +209,8 @@ template <int HD>
 __device__ __forceinline__ void issue_chunk_warp(const MmaAttnParams& p, __nv_bfloat16* ks, __nv_bfloat16* vs,
                                                  unsigned long long* bar, int c0, int lo, int hi, int kept, const int* bt,
                                                  const __nv_bfloat16* kbase, const __nv_bfloat16* vbase,
-                                                 size_t page_stride, int lane, const int* cached) {
+                                                 size_t page_stride, int lane, const int* cached,
+                                                 const SharedPages* group = nullptr) {
     const int ps = p.page_size, pages = CHUNK >> p.page_shift;
     const unsigned tile_bytes = (unsigned)(ps * HD * sizeof(__nv_bfloat16));
     int page = -1;
@@ -217,10 +218,10 @@ __device__ __forceinline__ void issue_chunk_warp(const MmaAttnParams& p, __nv_bf
         const int key0 = c0 + lane * ps;
         if (key0 <= hi && (key0 + ps - 1 >= lo || key0 < kept)) {
             const int lp = key0 >> p.page_shift;
-            page = cached != nullptr ? cached[lane] : (lp < p.bt_stride ? bt[lp] : -1);
+            page = cached != nullptr ? cached[lane] : (group != nullptr ? shared_page(*group, lp) : (lp < p.bt_stride ? bt[lp] : -1));
             if (page < 0 || page >= p.n_pages) {
+                if (group == nullptr || page != PAGE_UNSEEN) atomicOr(p.status, MX_STATUS_BAD_PAGE);
                 page = -1;
-                atomicOr(p.status, MX_STATUS_BAD_PAGE);
             }
         }
     }
@@ -271,10 +272,12 @@ attention_mma_kernel(const MmaAttnParams p) {
     const int tile = blockIdx.x, kh = blockIdx.y, split = blockIdx.z;
     // no tile list: tile i is the whole of sequence i (a batch of decoding requests), one look-up less
     int seq, tile_row0, q_start, q_len, ctx = 0;
+    SharedPages group_pages;                    // SHARED_KEYS
     if (KEYS == SHARED_KEYS) {
         const GroupTile found = find_group_tile(p.shared, p.cu_q, tile, TILE_ROWS, p.group, lane);
         if (found.tokens <= 0) return;
         seq = found.seq; tile_row0 = found.first; q_start = found.q_start; q_len = found.tokens;
+        group_pages = shared_pages_of(p.shared, found, p.block_tables, p.bt_stride, p.cu_q, p.context_lens, p.page_size, p.window);
     } else if (KEYS == OWN_KEYS && !NARROW) {
         const SequenceTile found = find_sequence_tile(p.shared, p.cu_q, tile, TILE_ROWS, p.group, lane);
         if (found.seq < 0) {
@@ -389,6 +392,10 @@ attention_mma_kernel(const MmaAttnParams p) {
     if (!NARROW && KEYS != ALL_KEYS) {
         for (int e = tid; e < min((c_end - c_begin) * chunk_pages, NARROW_TABLE); e += MMA_THREADS)
             narrow_table[e] = share_from + e < p.bt_stride ? bt[share_from + e] : -1;
+        if (KEYS == SHARED_KEYS)
+            for (int e = tid; e < min((c_end - c_begin) * chunk_pages, NARROW_TABLE); e += MMA_THREADS)
+                if (narrow_table[e] < 0 && (share_from + e + 1) * p.page_size > lo_tile)
+                    narrow_table[e] = shared_page_of_others(group_pages, share_from + e);
         __syncthreads();
     }
     if (NARROW && KEYS == OWN_KEYS) {
@@ -751,7 +758,8 @@ attention_mma_kernel(const MmaAttnParams p) {
             __nv_bfloat16* ks = stages + (size_t)(i % WIDE_STAGES) * STAGE_ELEMS;
             issue_chunk_warp<HD>(p, ks, ks + CHUNK * HD, &bars[i % WIDE_STAGES], chunk_of(ci) * CHUNK, lo_tile, hi_tile, kept, bt,
                                  kbase, vbase, page_stride, lane,
-                                 (i + 1) * chunk_pages <= NARROW_TABLE ? narrow_table + i * chunk_pages : nullptr);
+                                 (i + 1) * chunk_pages <= NARROW_TABLE ? narrow_table + i * chunk_pages : nullptr,
+                                 KEYS == SHARED_KEYS ? &group_pages : nullptr);
         } else if (ci < c_end) {
             __nv_bfloat16* ks = stages + (size_t)((ci - c_begin) % WIDE_STAGES) * STAGE_ELEMS;
             issue_chunk<HD>(p, ks, ks + CHUNK * HD, &bars[(ci - c_begin) % WIDE_STAGES], chunk_of(ci) * CHUNK, lo_tile,

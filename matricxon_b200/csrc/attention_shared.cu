@@ -5,7 +5,8 @@
 // scores q.k * scale, optionally capped; float softmax, with a sink in its denominator where the caller has one). The softmax
 // of a (token, head) is cut into parts over disjoint keys, each with its maximum m_i, its sum l_i of exp(score - m_i) and its
 // weighted values o_i, in float:
-//   shared parts   the keys below lens[sequence], through the block table of the group's first sequence. The rows of an MMA
+//   shared parts   the keys below lens[sequence], through the block table of the group's first sequence (under a window through
+//                  another one's where that one has given the page up: shared_prefix.cuh). The rows of an MMA
 //                  tile are (token, head) pairs of the whole group, whatever sequence a token is of;
 //   own parts      the keys from there on, through the sequence's own table;
 //   joined         m = max m_i, w_i = exp(m_i - m), out = sum w_i o_i / (sum w_i l_i + exp(sink - m)), rounded once.
@@ -31,7 +32,7 @@ constexpr int SH_ROWS_PER_WARP = SH_ROWS / SH_WARPS;
 struct SharedAttnParams {
     const void *q, *cache;
     float *part_o, *part_ml;
-    const int *block_tables, *cu_q;
+    const int *block_tables, *cu_q, *context_lens;
     int* status;
     long long n_pages;
     int q_stride, bt_stride, n_tokens, n_heads, n_kv_heads, group, head_dim, page_size, window, n_splits, part;
@@ -91,11 +92,13 @@ shared_simt_kernel(const SharedAttnParams p) {
     if (SHARED || !p.shared.beside) pdl_wait();
     pdl_trigger();
     int seq = 0, rows = 0, first_token = 0, first_row = 0;
+    SharedPages group_pages;                                  // SHARED
     if (SHARED) {
         const GroupTile found = find_group_tile(p.shared, p.cu_q, blockIdx.x, SH_ROWS, p.group, lane);
         if (found.tokens <= 0) return;
         seq = found.seq; first_token = found.q_start; first_row = found.first;
         rows = min(SH_ROWS, found.tokens * p.group - first_row);
+        group_pages = shared_pages_of(p.shared, found, p.block_tables, p.bt_stride, p.cu_q, p.context_lens, p.page_size, p.window);
     } else {
         const int parts = (p.group + SH_ROWS - 1) / SH_ROWS;
         first_token = blockIdx.x / parts;
@@ -140,10 +143,11 @@ shared_simt_kernel(const SharedAttnParams p) {
         const int key = c0 + lane, lp = key / p.page_size, offset = key - lp * p.page_size, run0 = key - key % E;
         int page = -1;
         if (run0 <= hi && run0 + E - 1 >= lo) {
-            if (lp < p.bt_stride) page = bt[lp];
+            if (SHARED) page = shared_page(group_pages, lp);
+            else if (lp < p.bt_stride) page = bt[lp];
             if (page < 0 || page >= p.n_pages) {
+                if (key >= lo && key <= hi && !(SHARED && page == PAGE_UNSEEN)) atomicOr(p.status, MX_STATUS_BAD_PAGE);
                 page = -1;
-                if (key >= lo && key <= hi) atomicOr(p.status, MX_STATUS_BAD_PAGE);
             }
         }
         // a warp a key
@@ -459,8 +463,8 @@ bool rows_aligned(const void* q, int q_stride, const void* cache) {
 }  // namespace
 
 int mx_attention_tc_shared(const void* q, int q_stride, const void* cache, long long n_pages, int page_size,
-                           const int* block_tables, int bt_stride, const int* cu_q, int n_tokens, int n_heads, int n_kv_heads,
-                           int window, float scale, float softcap, int n_tiles, int n_splits, float* part_o, float* part_ml,
+                           const int* block_tables, int bt_stride, const int* cu_q, const int* context_lens, int n_tokens,
+                           int n_heads, int n_kv_heads, int window, float scale, float softcap, int n_tiles, int n_splits, float* part_o, float* part_ml,
                            const SharedPrefixParams& shared, int* status, cudaStream_t stream);
 int mx_attention_mma_shared(const void* q, int q_stride, const void* cache, long long n_pages, int page_size,
                             const int* block_tables, int bt_stride, const int* cu_q, const int* context_lens, int n_heads,
@@ -504,7 +508,7 @@ extern "C" int mx_paged_attention_shared(const void* q, int dtype, int q_stride,
     const SharedPlan plan = make_plan(dtype, head_dim, page_size, rows_aligned(q, q_stride, cache), n_tokens, n_heads, n_kv_heads,
                                       n_seqs, n_groups, max_q_len, max_shared_len, max_own_len, n_sm);
     SharedAttnParams p;
-    p.q = q; p.cache = cache; p.block_tables = block_tables; p.cu_q = cu_q; p.status = status; p.n_pages = n_pages;
+    p.q = q; p.cache = cache; p.block_tables = block_tables; p.cu_q = cu_q; p.context_lens = context_lens; p.status = status; p.n_pages = n_pages;
     p.q_stride = q_stride; p.bt_stride = bt_stride; p.n_tokens = n_tokens; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads;
     p.group = n_heads / n_kv_heads; p.head_dim = head_dim; p.page_size = page_size; p.window = window; p.scale = scale;
     p.softcap = softcap;
@@ -518,9 +522,9 @@ extern "C" int mx_paged_attention_shared(const void* q, int dtype, int q_stride,
     int rc = MX_OK;
     if (plan.shared_parts > 0) {
         if (plan.path == 2) {
-            rc = mx_attention_tc_shared(q, q_stride, cache, n_pages, page_size, block_tables, bt_stride, cu_q, n_tokens, n_heads,
-                                        n_kv_heads, window, scale, softcap, plan.shared_tiles, plan.shared_parts, p.part_o, p.part_ml,
-                                        p.shared, status, stream);
+            rc = mx_attention_tc_shared(q, q_stride, cache, n_pages, page_size, block_tables, bt_stride, cu_q, context_lens,
+                                        n_tokens, n_heads, n_kv_heads, window, scale, softcap, plan.shared_tiles, plan.shared_parts,
+                                        p.part_o, p.part_ml, p.shared, status, stream);
         } else if (plan.path == 1) {
             rc = mx_attention_mma_shared(q, q_stride, cache, n_pages, page_size, block_tables, bt_stride, cu_q, context_lens,
                                          n_heads, n_kv_heads, head_dim, window, scale, softcap, true, false, plan.shared_tiles,

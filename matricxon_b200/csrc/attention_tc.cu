@@ -239,7 +239,7 @@ __device__ __forceinline__ unsigned at_pack(float lo, float hi) {
 }
 
 // SHARED: the tiles are of a group's tokens, which have their first keys in common, and the keys are those alone
-// (attention_shared.cu): a tile's tokens may come from many sequences, the pages are those of the group's first one, each row
+// (attention_shared.cu): a tile's tokens may come from many sequences, the pages are those of the group (shared_page), each row
 // has limits of its own, and what comes out are always parts.
 template <bool BIASED, bool SHARED>
 __global__ void __launch_bounds__(AT_THREADS, 1)
@@ -266,6 +266,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     const int tile = (int)(blockIdx.x / (unsigned)p.n_kv_heads);
     const int kh = (int)(blockIdx.x % (unsigned)p.n_kv_heads);
     int seq, tok0, q_start, q_len, ctx = 0;
+    SharedPages group_pages;                                        // SHARED
     if (SHARED) {
         // the queries come from the kernel before; once that has ended, the launch after this one may begin beside it
         pdl_wait();
@@ -274,6 +275,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         const GroupTile found = find_group_tile(p.shared, p.cu_q, tile, p.tokens_per_tile, 1, lane);
         if (found.tokens <= 0) return;                              // more blocks than tiles
         seq = found.seq; tok0 = found.first; q_start = found.q_start; q_len = found.tokens;
+        group_pages = shared_pages_of(p.shared, found, p.block_tables, p.bt_stride, p.cu_q, p.context_lens, p.page_size, p.window);
     } else {
         seq = p.tiles[2 * tile]; tok0 = p.tiles[2 * tile + 1];
         q_start = p.cu_q[seq];
@@ -322,17 +324,26 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         const int j = i / pages_per_chunk;
         return ((chunk_of(j) * AT_KEYS) >> p.page_shift) + (i - j * pages_per_chunk);
     };
-    // this tile's part of the block table, read once by each producer (entries beyond AT_TABLE stay in global memory)
-    auto read_table = [&](int* table) {
-        const int n_table = min(n_chunks * pages_per_chunk, AT_TABLE);
+    // this tile's part of the block table, read once by each producer (entries beyond AT_TABLE stay in global memory; of a
+    // group's pages, which may have to be looked for, the next ones `from` there take the place of those that are done with)
+    auto read_table = [&](int* table, int from) {
+        const int n_table = min(n_chunks * pages_per_chunk - from, AT_TABLE);
         for (int i = lane; i < n_table; i += 32) {
-            const int lp = logical_page(i);
+            const int lp = logical_page(from + i);
             table[i] = lp < p.bt_stride ? bt[lp] : -1;
         }
+        // (looking for pages in the loop above would have its loads wait for one another: 202 us where this takes 192, 128
+        // requests on 32,768 keys)
+        if (SHARED)
+            for (int i = lane; i < n_table; i += 32) {
+                const int lp = logical_page(from + i);
+                if (table[i] < 0 && (lp + 1) * p.page_size > lo_tile) table[i] = shared_page_of_others(group_pages, lp);
+            }
         __syncwarp();
     };
     // the keys (or the values) of chunk j into stage j % AT_STAGES: lane pg brings page pg
-    auto bring = [&](int j, bool keys, const int* table) {
+    auto bring = [&](int j, bool keys, int* table) {
+        if (SHARED && j > 0 && j * pages_per_chunk % AT_TABLE == 0) read_table(table, j * pages_per_chunk);
         const int s = j % AT_STAGES;
         unsigned long long* full = keys ? &sh.k_full[s] : &sh.v_full[s];
         const int c0 = chunk_of(j) * AT_KEYS;
@@ -342,10 +353,10 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
             if (key0 <= hi_tile && (key0 + p.page_size - 1 >= lo_tile || key0 < p.keep)) {
                 const int i = j * pages_per_chunk + lane;
                 const int lp = logical_page(i);
-                page = i < AT_TABLE ? table[i] : (lp < p.bt_stride ? bt[lp] : -1);
+                page = SHARED ? table[i % AT_TABLE] : (i < AT_TABLE ? table[i] : (lp < p.bt_stride ? bt[lp] : -1));
                 if (page < 0 || page >= p.n_pages) {
+                    if (keys && !(SHARED && page == PAGE_UNSEEN)) atomicOr(p.status, MX_STATUS_BAD_PAGE);
                     page = -1;
-                    if (keys) atomicOr(p.status, MX_STATUS_BAD_PAGE);
                 }
             }
         }
@@ -388,7 +399,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
             tma_4d(q_tile + AT_TILE, &q_map, 64, 0, kh, q_start + tok0, &sh.q_full);
         }
         __syncwarp();
-        read_table(table_k);
+        read_table(table_k, 0);
         bring(0, true, table_k);
     } else if (warp == AT_MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&sh.tmem_base)),
@@ -396,7 +407,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     } else if (warp == AT_VALUE_WARP) {
-        read_table(table_v);
+        read_table(table_v, 0);
     } else {
         // value stages start as zeros: a page that is never fetched must not hold NaN bit patterns
         for (int i = tid; i < AT_STAGES * 2 * AT_TILE / 16; i += AT_SOFTMAX_THREADS)
@@ -884,15 +895,15 @@ extern "C" int mx_paged_attention_tc(const void* q, int q_stride, const void* ca
 // The keys that groups of sequences have in common, for attention_shared.cu: a tile holds 128 / group tokens of one group.
 // Parts 0 .. n_splits - 1 of `part_o` and `part_ml` (of shared.n_parts a token and head) are written for every token of a group.
 int mx_attention_tc_shared(const void* q, int q_stride, const void* cache, long long n_pages, int page_size,
-                           const int* block_tables, int bt_stride, const int* cu_q, int n_tokens, int n_heads, int n_kv_heads,
-                           int window, float scale, float softcap, int n_tiles, int n_splits, float* part_o, float* part_ml,
+                           const int* block_tables, int bt_stride, const int* cu_q, const int* context_lens, int n_tokens,
+                           int n_heads, int n_kv_heads, int window, float scale, float softcap, int n_tiles, int n_splits, float* part_o, float* part_ml,
                            const SharedPrefixParams& shared, int* status, cudaStream_t stream) {
     const int group = n_heads / n_kv_heads;
     CUtensorMap q_map, k_map, v_map;
     const int mapped = at_make_maps(&q_map, &k_map, &v_map, q, q_stride, cache, n_pages, page_size, n_tokens, n_kv_heads, group);
     if (mapped != MX_OK) return mapped;
     AtParams p = {};
-    p.block_tables = block_tables; p.cu_q = cu_q; p.part_o = part_o; p.part_ml = part_ml; p.n_splits = n_splits;
+    p.block_tables = block_tables; p.cu_q = cu_q; p.context_lens = context_lens; p.part_o = part_o; p.part_ml = part_ml; p.n_splits = n_splits;
     p.status = status; p.n_pages = n_pages; p.n_tiles = n_tiles; p.bt_stride = bt_stride; p.n_heads = n_heads;
     p.n_kv_heads = n_kv_heads; p.group = group; p.tokens_per_tile = AT_ROWS / group; p.page_size = page_size;
     p.page_shift = page_size == 16 ? 4 : 5; p.window = window; p.scale_log2 = scale * 1.4426950408889634f;

@@ -2,7 +2,8 @@
 //
 // The step's sequences lie in groups one after another: group g holds sequences first[g] .. first[g + 1] - 1. Sequence s reads
 // its keys below lens[s] through the block table of its group's first sequence, together with the rest of the group, and its
-// keys from lens[s] on through its own.
+// keys from lens[s] on through its own. Under a window (or blocks) the first sequence may have given up pages that others of
+// the group still see: those are read through the first one of these that has to hold them (shared_page).
 #pragma once
 
 #include "common.cuh"
@@ -57,7 +58,7 @@ __device__ __forceinline__ KeyRange shared_keys_of_tokens(const SharedPrefixPara
 }
 
 struct GroupTile {
-    int seq;                 // the group's first sequence
+    int seq, end;            // the group's sequences: seq .. end - 1
     int q_start, tokens;     // the group's tokens; none: there is no such tile
     int first;               // where the tile starts among their rows
 };
@@ -65,15 +66,16 @@ struct GroupTile {
 // Tile `tile` of the groups' rows (`rows` a token) cut into tiles of `per_tile` rows, group after group; by a whole warp. The lists live on the
 // device, so a captured step may be replayed with other groups; a launch has blocks for the most tiles that there can be.
 __device__ __forceinline__ GroupTile find_group_tile(const SharedPrefixParams& p, const int* cu_q, int tile, int per_tile, int rows, int lane) {
-    GroupTile found = {0, 0, 0, 0};
+    GroupTile found = {0, 0, 0, 0, 0};
     int before = 0;
     for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
         const int g = g0 + lane;
-        int seq = 0, start = 0, tokens = 0;
+        int seq = 0, end = 0, start = 0, tokens = 0;
         if (g < p.n_groups) {
             seq = min(max(p.first[g], 0), p.n_seqs);
+            end = min(max(p.first[g + 1], 0), p.n_seqs);
             start = min(cu_q[seq], p.n_tokens);
-            tokens = min(cu_q[min(max(p.first[g + 1], 0), p.n_seqs)], p.n_tokens) - start;
+            tokens = min(cu_q[end], p.n_tokens) - start;
         }
         const int tiles = tokens > 0 ? (tokens * rows + per_tile - 1) / per_tile : 0;
         int through = tiles;
@@ -86,6 +88,7 @@ __device__ __forceinline__ GroupTile find_group_tile(const SharedPrefixParams& p
         if (past) {
             const int at = __ffs(past) - 1;
             found.seq = __shfl_sync(0xffffffffu, seq, at);
+            found.end = __shfl_sync(0xffffffffu, end, at);
             found.q_start = __shfl_sync(0xffffffffu, start, at);
             found.tokens = __shfl_sync(0xffffffffu, tokens, at);
             found.first = (tile - before - __shfl_sync(0xffffffffu, through - tiles, at)) * per_tile;
@@ -94,6 +97,42 @@ __device__ __forceinline__ GroupTile find_group_tile(const SharedPrefixParams& p
         before += __shfl_sync(0xffffffffu, through, 31);
     }
     return found;
+}
+
+// Where a page of a group's shared keys is looked up.
+struct SharedPages {
+    const int *block_tables, *cu_q, *context_lens, *lens;
+    int bt_stride, page_size, window, seq, end;       // sequences seq .. end - 1
+};
+constexpr int PAGE_UNSEEN = -2;                       // no page, and no query of the group sees a key of it
+
+__device__ __forceinline__ SharedPages shared_pages_of(const SharedPrefixParams& p, const GroupTile& group, const int* block_tables,
+                                                       int bt_stride, const int* cu_q, const int* context_lens, int page_size, int window) {
+    return SharedPages{block_tables, cu_q, context_lens, p.lens, bt_stride, page_size, window, group.seq, group.end};
+}
+
+// A page that the group's first sequence has no entry for. That is in order where it sees none of the page's keys any more.
+// The page is then that of the first sequence that sees one and shares the whole page (of a page that its shared keys fill in
+// part it has a copy of its own, whose first slots nobody fills). -1: there is no such sequence, though the page is seen.
+// A sequence's lengths are two loads at one place for a whole warp, so a warp walks a group of 128 in a few us; only groups
+// whose first sequence has moved on come here.
+static __device__ __forceinline__ int shared_page_of_others(const SharedPages& g, int lp) {
+    const long long begin = (long long)lp * g.page_size, last = begin + g.page_size - 1;
+    bool seen = false;
+    for (int s = g.seq; s < g.end; ++s) {
+        const int context = g.context_lens[s], tokens = g.cu_q[s + 1] - g.cu_q[s], shared = g.lens[s];
+        const int low = first_visible_key(context, g.window), high = min(context + tokens, shared) - 1;
+        if (tokens <= 0 || low > last || high < begin || high < low) continue;
+        if (s == g.seq) return -1;
+        seen = true;
+        if (last < shared) return lp < g.bt_stride ? max(g.block_tables[(size_t)s * g.bt_stride + lp], -1) : -1;
+    }
+    return seen ? -1 : PAGE_UNSEEN;
+}
+
+__device__ __forceinline__ int shared_page(const SharedPages& g, int lp) {
+    const int page = lp < g.bt_stride ? g.block_tables[(size_t)g.seq * g.bt_stride + lp] : -1;
+    return page >= 0 ? page : shared_page_of_others(g, lp);
 }
 
 // The same over the sequences' own (token, head) rows, tiles of `rows` rows of `group` a token: (sequence, first row).

@@ -710,7 +710,10 @@ def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, 
     Sequences ``shared_first[g] .. shared_first[g + 1] - 1`` (int32 [groups + 1], from 0 to the number of sequences) are
     group g. Sequence s reads its keys below ``shared_lens[s]`` (int32, one per sequence; 0: none) through the block table
     of its group's first sequence, the others through its own, so the tables of ``paged_attention`` serve as they are: shared
-    pages stand in every table of the group. ``q``, ``out``, ``window``, ``softcap`` and ``sink`` as in ``paged_attention``;
+    pages stand in every table of the group. Under a window or blocks these may leave out (-1) what their sequence no longer
+    sees, as ``step_tables`` and the cache manager do: a shared page that the first sequence sees no key of any more is read
+    through the first other one that does. A page that the shared keys fill in part is the first sequence's alone and has to
+    be in its table while any sequence sees those keys (otherwise the status word is set). ``q``, ``out``, ``window``, ``softcap`` and ``sink`` as in ``paged_attention``;
     sequence s brings rows ``cu_q[s] .. cu_q[s + 1] - 1``, row i of it at position ``context_lens[s] + i``, which
     ``positions`` and ``tok_seq`` repeat row by row. Rows from ``cu_q[-1]`` on are left alone.
 

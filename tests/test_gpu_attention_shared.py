@@ -351,3 +351,67 @@ def test_refusals():
     with pytest.raises(KernelLibraryError):
         odd.run()
     assert kernels.describe_status(16) != "no error"
+
+
+def out_of_sight(step, window):
+    """The step's tables without what no query of a sequence sees any more, as the cache manager and step_tables leave them."""
+    tables = [list(row) for row in step.tables]
+    for row, context in zip(tables, step.context):
+        low = max(0, context - window + 1) if window > 0 else context - context % -window
+        row[:low // step.page] = [-1] * (low // step.page)
+    step.d["tables"] = ints(tables)
+    return step
+
+
+WINDOWED = {
+    "longest first": [(512, [(900, 1), (0, 1), (300, 1), (80, 1)])],
+    "longest in the middle": [(512, [(100, 1), (900, 1), (20, 1)]), (0, [(40, 1)])],
+    "portions": [(512, [(500, 20), (3, 1), (0, 33), (130, 2)])],
+    "nobody sees the first pages": [(1056, [(310, 1), (120, 1), (200, 1)])],
+    "shared keys that fill no page": [(517, [(40, 1), (0, 1), (90, 3)])],
+    "first ones without tokens": [(512, [(900, 0), (0, 0), (600, 1), (10, 1)])],
+    "more requests than a warp": [(256, [(700 - 13 * i, 1) for i in range(50)])],
+}
+
+
+@pytest.mark.parametrize("shape", [SHAPES[0], SHAPES[1], SHAPES[4], SHAPES[5], SHAPES[7], SHAPES[8], SHAPES[10], SHAPES[12]], ids=str)
+@pytest.mark.parametrize("window", [300, 77, -256])
+@pytest.mark.parametrize("name", WINDOWED)
+def test_pages_that_the_first_sequence_no_longer_holds(shape, window, name):
+    """Tables of a window: the group's first sequence has given pages back that others of the group still see."""
+    groups = WINDOWED[name]
+    if shape[3] == 24:
+        groups = [(shared // 24 * 24, members) for shared, members in groups]
+    step = out_of_sight(Step(groups, *shape, seed=len(name)), window)
+    close(step, step.run(window=window), window=window)
+
+
+@pytest.mark.parametrize("shape", [SHAPES[0], SHAPES[5], SHAPES[10]], ids=str)
+def test_pages_between_that_nobody_sees(shape):
+    """Shared lengths that differ within a group: under a window its sequences see stretches with a gap between them."""
+    step = out_of_sight(Step([(96, [(404, 1), (4, 1), (20, 1)])], *shape, seed=2), 50)
+    step.d["lens"] = ints([500, 96, 96])
+    close(step, step.run(window=50, max_shared_len=500), window=50)
+
+
+@pytest.mark.parametrize("shape", [SHAPES[0], SHAPES[5], SHAPES[10]], ids=str)
+def test_a_page_that_all_have_lost_is_reported(shape):
+    step = out_of_sight(Step([(512, [(900, 1), (0, 1), (80, 1)])], *shape, seed=3), 300)
+    step.d["tables"][1:, 300 // step.page] = -1
+    step.run(window=300)
+    assert step.d["status"].item() == 4
+
+
+@pytest.mark.parametrize("shape", [SHAPES[0], SHAPES[5], SHAPES[10]], ids=str)
+def test_a_lost_page_that_the_shared_keys_fill_in_part_is_reported(shape):
+    """Only the first sequence's page holds them; the others have a copy of their own, of which nobody says what is in it."""
+    step = out_of_sight(Step([(517, [(900, 1), (0, 1)])], *shape, seed=3), 300)
+    step.run(window=300)
+    assert step.d["status"].item() == 4
+
+
+@pytest.mark.parametrize("shape", [SHAPES[0], SHAPES[5]], ids=str)
+def test_lost_pages_beyond_what_a_block_keeps_of_its_table(shape):
+    """More pages in one part than a block reads ahead."""
+    step = out_of_sight(Step([(40000, [(30000, 1), (0, 1), (7, 1)])], *shape, seed=5), 39000)
+    close(step, step.run(window=39000, max_shared_len=1), window=39000)

@@ -243,3 +243,96 @@ def test_two_streams_at_once():
                 assert case.run() == expected
             torch.cuda.synchronize()
     assert all(step.d["status"].item() == 0 for step in attention)
+
+
+@pytest.mark.parametrize("chained", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype,window", [(8, 2, 128, 16, torch.bfloat16, 64), (8, 2, 128, 16, torch.bfloat16, -96),
+                                                                  (16, 4, 64, 8, torch.bfloat16, 40), (6, 2, 80, 16, torch.bfloat16, 64),
+                                                                  (24, 2, 128, 16, torch.float32, 50)])
+def test_a_decoding_loop_under_a_window(chained, heads, kv_heads, dim, page, dtype, window):
+    """Requests on one prefix, the longest first: attention on the tables that the step's kernel writes, which leave out what a
+    request no longer sees. Against one softmax over each request's keys, in 64 bits, by its bounds."""
+    from matricxon_b200.ops import kernels
+
+    prefix, n, steps = 160, 6, 8
+    own = [150, 30, 0, 70, 15, 1]
+    context = [prefix + k for k in own]
+    width, n_pages = 45, 400
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    ints = lambda values: torch.tensor(values, dtype=torch.int32, device=DEV)  # noqa: E731
+    history = [(torch.randn(context[s] + steps, kv_heads, dim, generator=gen, device=DEV).to(dtype),
+                torch.randn(context[s] + steps, kv_heads, dim, generator=gen, device=DEV).to(dtype)) for s in range(n)]
+    for k, v in history[1:]:
+        k[:prefix], v[:prefix] = history[0][0][:prefix], history[0][1][:prefix]
+    cache = torch.full((n_pages, 2, kv_heads, page, dim), float("nan"), dtype=dtype, device=DEV)
+    values = cache[:, 1].view(n_pages, kv_heads, dim, page)
+    pages = torch.randperm(n_pages, generator=torch.Generator().manual_seed(1)).tolist()
+    tables = [[-1] * width for _ in range(n)]
+    for s in range(n):
+        for k in range(prefix // page if s else 0, -(-context[s] // page)):
+            tables[s][k] = pages.pop()
+    for s in range(n):
+        for p in range(prefix if s else 0, context[s]):
+            cache[tables[s][p // page], 0, :, p % page] = history[s][0][p]
+            values[tables[s][p // page], :, :, p % page] = history[s][1][p]
+    tables, free = ints(tables), ints(pages)
+    shared_rows, shared_pages = ints([-1] + [0] * (n - 1)), ints([0] + [prefix // page] * (n - 1))
+    lengths, status = ints(context), ints([0])
+    out = {name: torch.empty(size, dtype=torch.int32, device=DEV) for name, size in
+           (("positions", n), ("tok_seq", n), ("cu_q", n + 1), ("slots", n), ("taken", 1))}
+    block_tables, taken_all = torch.empty(n, width, dtype=torch.int32, device=DEV), ints([0])
+    q, key, value = (torch.zeros(n, h * dim, dtype=dtype, device=DEV) for h in (heads, kv_heads, kv_heads))
+    attended = torch.empty(n, heads * dim, dtype=dtype, device=DEV)
+    q_lens, n_free, first, shared_lens = ints([1] * n), ints([len(pages)]), ints([0, n]), ints([prefix] * n)
+    places = torch.arange(free.numel(), device=DEV)
+
+    def step():
+        kernels.step_tables(q_lens, lengths, None, tables, free, n_free, page, n_pages, out["positions"], out["tok_seq"], out["cu_q"],
+                            out["slots"], block_tables, out["taken"], status, shared_rows=shared_rows, shared_pages=shared_pages, window=window)
+        at, inside = out["slots"].long() // page, out["slots"].long() % page
+        cache[:, 0].transpose(1, 2)[at, inside] = key.view(n, kv_heads, dim)
+        values.permute(0, 3, 1, 2)[at, inside] = value.view(n, kv_heads, dim)
+        kernels.paged_attention_shared(q, q.stride(0), cache, block_tables, out["cu_q"], lengths, out["tok_seq"], out["positions"],
+                                       first, shared_lens, n, heads, kv_heads, dim, window, dim ** -0.5, attended, status, max_q_len=1,
+                                       max_shared_len=prefix, max_own_len=256)
+        lengths.add_(1)
+        free.copy_(free[(places + out["taken"]) % free.numel()])
+        taken_all.add_(out["taken"])
+
+    keep = [t.clone() for t in (tables, free, lengths, cache)]
+    step()
+    for tensor, kept in zip((tables, free, lengths, cache), keep):
+        tensor.copy_(kept)
+    status.zero_()
+    taken_all.zero_()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    kernels.set_chained_launch(chained)
+    try:
+        with torch.cuda.graph(graph):
+            step()
+    finally:
+        kernels.set_chained_launch(False)
+    half, out_half = torch.finfo(torch.float32).eps / 2, torch.finfo(dtype).eps / 2
+    for i in range(steps):
+        q.copy_((1.5 * torch.randn(n, heads * dim, generator=gen, device=DEV)).to(dtype))
+        for s in range(n):
+            key[s], value[s] = history[s][0][context[s] + i].view(-1), history[s][1][context[s] + i].view(-1)
+        graph.replay()
+        for s in range(n):
+            position = context[s] + i
+            low = max(0, position - window + 1) if window > 0 else position - position % -window
+            k, v = (t[low:position + 1].double() for t in history[s])
+            rows = q[s].double().view(kv_heads, heads // kv_heads, dim)
+            weights = torch.softmax(torch.einsum("kgd,jkd->kgj", rows, k) * dim ** -0.5, -1)
+            size = torch.einsum("kgd,jkd->kgj", rows.abs(), k.abs()) * dim ** -0.5
+            ref = torch.einsum("kgj,jkd->kgd", weights, v)
+            sizes = torch.einsum("kgj,jkd->kgd", weights, v.abs())
+            # the bound of test_gpu_attention_shared.py: scores, exponentials, two sums of n weights; a weight rounded to
+            # bfloat16 before it meets its value; the result rounded once
+            off = (2 * (dim + 4) * half * size.amax(-1) + 32 * half)[..., None] * 2 + (2 * k.shape[0] + 16) * half
+            bound = (off + (out_half if dtype == torch.bfloat16 else 0.0)) * sizes + out_half * ref.abs()
+            assert ((attended[s].double().view_as(ref) - ref).abs() <= bound).all()
+            assert block_tables[s, :low // page].max().item() < 0 if low >= page else True
+    assert status.item() == 0
+    assert taken_all.item() == sum(-(-(c + steps) // page) - -(-c // page) for c in context)
