@@ -604,7 +604,7 @@ attention_mma_kernel(const MmaAttnParams p) {
                 o[nb][2] *= alpha[1]; o[nb][3] *= alpha[1];
             }
         }
-        if (first_key[NCH - 1] + CHUNK - 1 <= hi_tile) {
+        if (first_key[NCH - 1] + CHUNK - 1 <= hi_tile && (KEYS == ALL_KEYS || first_key[0] >= lo_tile)) {
 #pragma unroll
             for (int nb0 = 0; nb0 < NB; nb0 += 4)
 #pragma unroll
@@ -621,14 +621,17 @@ attention_mma_kernel(const MmaAttnParams p) {
                         mma_bf16(o[nb0 + j], pa[ch][1][0], pa[ch][1][1], pa[ch][1][2], pa[ch][1][3], vf[j].z, vf[j].w);
                 }
         } else {
-            // slots beyond the newest key hold no data yet: keep them out of the product
+            // slots beyond the newest key hold no data yet: keep them out of the product. So may those before a sequence's
+            // own keys, in the page where the shared ones end
             unsigned keep[NCH][4];
 #pragma unroll
             for (int ch = 0; ch < NCH; ++ch) {
                 const int vkey0 = first_key[ch] + 8 * t;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const bool lo_ok = vkey0 + 2 * w <= hi_tile, hi_ok = vkey0 + 2 * w + 1 <= hi_tile;
+                    const int key = vkey0 + 2 * w;
+                    const bool lo_ok = key <= hi_tile && (KEYS == ALL_KEYS || key >= lo_tile);
+                    const bool hi_ok = key + 1 <= hi_tile && (KEYS == ALL_KEYS || key + 1 >= lo_tile);
                     keep[ch][w] = (lo_ok ? 0x0000ffffu : 0u) | (hi_ok ? 0xffff0000u : 0u);
                 }
             }

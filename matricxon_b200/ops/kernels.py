@@ -720,8 +720,9 @@ def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, 
     ``max_q_len``: no sequence brings more tokens, and all together at most ``n_tokens`` (otherwise the status word is set). ``max_shared_len``,
     ``max_own_len`` (keys that a sequence shares, and does not) are for sizing: with other numbers the result is the same
     up to rounding. All three are host numbers, so that a captured step can be replayed with other lengths and groups
-    below them. ``scratch`` (float32) is taken from torch's allocator where none is given. The keys and values that any
-    token of a group sees have to be finite."""
+    below them. ``scratch`` (float32) is taken from torch's allocator where none is given. The shared keys and values have to be
+    finite on all pages from the first to the last that any token of a group sees, and so do the own ones that a sequence sees;
+    other slots may hold anything, those of a sequence's first own page before its own keys too."""
     here, code = _here("q", q), dtype_code(q.dtype)
     n_seqs = context_lens.numel()
     _need_all(here, q.dtype, ("cache", cache, -1))

@@ -415,3 +415,25 @@ def test_lost_pages_beyond_what_a_block_keeps_of_its_table(shape):
     """More pages in one part than a block reads ahead."""
     step = out_of_sight(Step([(40000, [(30000, 1), (0, 1), (7, 1)])], *shape, seed=5), 39000)
     close(step, step.run(window=39000, max_shared_len=1), window=39000)
+
+
+def forget_tails(step):
+    """The slots of a sequence's first own page that lie before its own keys, NaN in all but the group's first sequence's."""
+    cache = step.d["cache"]
+    keys, values = cache[:, 0], cache[:, 1].view(cache.shape[0], step.kv_heads, step.dim, step.page)
+    for s, shared in enumerate(step.lens):
+        tail = shared % step.page
+        if tail and s not in step.first and shared // step.page < len(step.tables[s]) and step.tables[s][shared // step.page] >= 0:
+            page = step.tables[s][shared // step.page]
+            keys[page, :, :tail] = float("nan")
+            values[page, :, :, :tail] = float("nan")
+    return step
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("masks", [{}, {"window": 40}, {"softcap": 5.0}], ids=str)
+@pytest.mark.parametrize("groups", [[(133, [(0, 1), (9, 1), (50, 1), (0, 1)])], [(133, [(0, 1), (9, 3), (50, 21), (0, 70)]), (5, [(1, 1), (90, 1)])],
+                                    [(257, [(0, 2)] * 9), (1, [(300, 1)] * 3)]], ids=["narrow", "portions", "one key over"])
+def test_slots_before_a_sequences_own_keys_hold_anything(shape, masks, groups):
+    step = forget_tails(Step(groups, *shape, seed=11))
+    close(step, step.run(**masks), **masks)
