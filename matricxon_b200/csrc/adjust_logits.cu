@@ -18,6 +18,9 @@
 // place in the list among a token's biases says which one holds. What a phase reads it asks for eight at a time.
 // Where a row has many blocks and a long list, a kernel beside deals the ids out to the stretches first, so that each is looked
 // at once, not by every block of the row.
+// Offsets live on the device, where a captured call may find others than those it was captured with: a row's part of a list is
+// what lies inside the list. Offsets that fall (parts of rows that overlap) have no place each in the dealt ids; every block
+// then reads its row's list.
 // 256 rows of 131,071 scores, a third of them allowed, with 6,144 ids each: 90 us (a copy of the scores takes 47), 121 with every
 // block reading the whole list, 92 with a kernel after this one that gathers each row's list in a hash table. What is left
 // above the copy are the atomics: shared memory takes some 0.75 lanes of them a cycle and SM, whatever words they go to.
@@ -39,6 +42,7 @@ struct AdjustParams {
     float* out;
     long long row_stride, out_stride;
     int vocab, mask_width, n_masks;
+    long long n_ids, n_biases;                       // sizes of the lists of all rows
     const int *token_offsets, *token_ids, *bias_offsets, *bias_ids, *mask_words, *mask_rows, *pending;
     const float *repeat, *presence, *frequency, *bias_values;
     int stretch;                                     // scores of a block
@@ -49,6 +53,17 @@ __device__ __forceinline__ const unsigned* mask_of(const AdjustParams& p, int ro
     if (p.mask_words == nullptr) return nullptr;
     const int at = p.mask_rows ? p.mask_rows[row] : row;
     return at >= 0 && at < p.n_masks ? reinterpret_cast<const unsigned*>(p.mask_words) + (size_t)at * p.mask_width : nullptr;
+}
+
+// Where a row's part of a list of `size` begins, and how long it is.
+struct Part {
+    int first, count;
+};
+__device__ __forceinline__ int within(int offset, long long size) { return (int)min(max((long long)offset, 0LL), size); }
+__device__ __forceinline__ Part part_of(const int* offsets, int row, long long size) {
+    if (offsets == nullptr) return Part{0, 0};
+    const int first = within(offsets[row], size);
+    return Part{first, max(within(offsets[row + 1], size) - first, 0)};
 }
 
 __device__ __forceinline__ void load_four(const float* from, float* x) {
@@ -72,9 +87,9 @@ __global__ void __launch_bounds__(DEAL_THREADS) deal_ids_kernel(const AdjustPara
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
     pdl_wait();
     pdl_trigger();                                    // the scores' kernel begins beside this one
-    const int first = p.token_offsets ? p.token_offsets[row] : 0, last = p.token_offsets ? p.token_offsets[row + 1] : 0;
-    const int pending = p.pending ? p.pending[row] : -1, shift = shift_of(p, row);
-    const int n = max(last - first, 0) + 1, log_stretch = 31 - __clz(p.stretch);       // a power of two
+    const Part list = part_of(p.token_offsets, row, p.n_ids);
+    const int first = list.first, pending = p.pending ? p.pending[row] : -1, shift = shift_of(p, row);
+    const int n = list.count + 1, log_stretch = 31 - __clz(p.stretch);       // a power of two
     // the stretches of ids k0 + tid, + DEAL_THREADS, ... (-1: none)
     auto ahead = [&](int k0, int* id, int* to) {
 #pragma unroll
@@ -86,10 +101,17 @@ __global__ void __launch_bounds__(DEAL_THREADS) deal_ids_kernel(const AdjustPara
         for (int e = 0; e < AL_AHEAD; ++e) to[e] = id[e] >= 0 && id[e] < p.vocab ? (id[e] + shift) >> log_stretch : -1;
     };
     int id[AL_AHEAD], to[AL_AHEAD];
+    ahead(0, id, to);
     for (int i = tid; i < n_blocks; i += DEAL_THREADS) count[i] = 0;
-    __syncthreads();
+    bool falls = false;
+    for (int i = tid; i < (int)gridDim.x; i += DEAL_THREADS)
+        falls = falls || within(p.token_offsets[i + 1], p.n_ids) < within(p.token_offsets[i], p.n_ids);
+    if (__syncthreads_or(falls)) {
+        if (tid == 0) p.dealt_from[(size_t)row * (n_blocks + 1)] = -1;        // nothing is dealt out
+        return;
+    }
     for (int k0 = 0; k0 < n; k0 += AL_AHEAD * DEAL_THREADS) {
-        ahead(k0, id, to);
+        if (k0 > 0) ahead(k0, id, to);
 #pragma unroll
         for (int e = 0; e < AL_AHEAD; ++e)
             if (to[e] >= 0) atomicAdd(&count[to[e]], 1);
@@ -204,22 +226,20 @@ __global__ void __launch_bounds__(AL_THREADS, 5) adjust_logits_kernel(const Adju
     // ---- the listed tokens
     const float repeat = p.repeat ? p.repeat[row] : 1.f, presence = p.presence ? p.presence[row] : 0.f;
     const float frequency = p.frequency ? p.frequency[row] : 0.f;
-    const int bias_first = p.bias_offsets ? p.bias_offsets[row] : 0, bias_last = p.bias_offsets ? p.bias_offsets[row + 1] : 0;
+    const Part biases = part_of(p.bias_offsets, row, p.n_biases);
     const unsigned to_place = (unsigned)(shift - begin), n = (unsigned)(end - begin);
-    const int* ids = p.token_ids;
-    int n_ids = 0, pending = -1;
+    const Part list = part_of(p.token_offsets, row, p.n_ids);
+    const int* ids = p.token_ids + list.first;
+    int n_ids = list.count, pending = p.pending ? p.pending[row] : -1;
     if (p.dealt != nullptr) {
         pdl_wait();                                   // the ids have been dealt out
-        const int* from = after_wait(p.dealt_from) + (size_t)row * (gridDim.x + 1) + blockIdx.x;
-        const int before = from[0];
-        n_ids = from[1] - before;
-        ids = after_wait(p.dealt) + (p.token_offsets ? p.token_offsets[row] : 0) + row + before;
-    } else {
-        if (p.token_offsets) {
-            ids += p.token_offsets[row];
-            n_ids = max(0, p.token_offsets[row + 1] - p.token_offsets[row]);
+        const int* from = after_wait(p.dealt_from) + (size_t)row * (gridDim.x + 1);
+        const int dealt = from[0], before = from[blockIdx.x], behind = from[blockIdx.x + 1];
+        if (dealt >= 0) {
+            n_ids = behind - before;
+            ids = after_wait(p.dealt) + (size_t)list.first + row + before;
+            pending = -1;                             // among them
         }
-        if (p.pending) pending = p.pending[row];
     }
     // places in the stretch of ids k0 + tid, + AL_THREADS, ... of a list (n or more: elsewhere)
     auto ahead = [&](const int* list, int count, int last_id, int k0, unsigned* at) {
@@ -262,8 +282,8 @@ __global__ void __launch_bounds__(AL_THREADS, 5) adjust_logits_kernel(const Adju
             }
         }
     }
-    if (bias_last > bias_first) {
-        const int n_biases = bias_last - bias_first;
+    if (biases.count > 0) {
+        const int bias_first = biases.first, n_biases = biases.count;
         ahead(p.bias_ids + bias_first, n_biases, -1, 0, at);
         bool here = n_biases > AL_AHEAD * AL_THREADS;
 #pragma unroll
@@ -320,11 +340,11 @@ extern "C" long long mx_adjust_logits_scratch(long long n_ids, int n_rows, int v
     return 4 * (n_ids + n_rows + n_rows * (blocks_of(n_rows, vocab) + 1));
 }
 
-// n_ids: how many there are of all rows together (the size of token_ids).
+// n_ids, n_biases: how many there are of all rows together (the sizes of token_ids and bias_ids).
 extern "C" int mx_adjust_logits(const void* logits, int dtype, long long row_stride, float* out, long long out_stride, int n_rows,
                                 int vocab, const int* token_offsets, const int* token_ids, long long n_ids, const float* repeat,
                                 const float* presence, const float* frequency, const int* bias_offsets, const int* bias_ids,
-                                const float* bias_values, const int* mask_words, int n_masks, int mask_width,
+                                const float* bias_values, long long n_biases, const int* mask_words, int n_masks, int mask_width,
                                 const int* mask_rows, const int* pending, int* scratch, cudaStream_t stream) {
     if (n_rows <= 0) return MX_OK;
     if (n_rows > 65535) MX_REFUSE("adjust logits: %d rows exceed the grid", n_rows);
@@ -335,6 +355,7 @@ extern "C" int mx_adjust_logits(const void* logits, int dtype, long long row_str
     p.mask_width = mask_width; p.n_masks = mask_words ? n_masks : 0; p.token_offsets = token_offsets; p.token_ids = token_ids;
     p.bias_offsets = bias_offsets; p.bias_ids = bias_ids; p.mask_words = mask_words; p.mask_rows = mask_rows; p.pending = pending;
     p.repeat = repeat; p.presence = presence; p.frequency = frequency; p.bias_values = bias_values;
+    p.n_ids = n_ids; p.n_biases = n_biases;
     p.stretch = stretch_of(n_rows, vocab);
     p.dealt = p.dealt_from = nullptr;
     const int n_blocks = (int)blocks_of(n_rows, vocab);

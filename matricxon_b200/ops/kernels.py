@@ -833,7 +833,8 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, token_offsets: torch.
     (float32 [rows]). ``bias_values`` (float32) are added at ``bias_ids``, row r's at ``bias_offsets[r]:bias_offsets[r + 1]``; of
     two of one token the later one counts. ``mask_words`` (int32 [masks, words]): bit v % 32 of word v / 32 says whether
     token v may be taken; a score that may not becomes -infinity. Row r goes by mask ``mask_rows[r]`` (a number that names no
-    mask, as -1: none), or by mask r where there is no ``mask_rows``. Ids outside the vocabulary are passed over. Rows of ``logits`` and ``out`` may be
+    mask, as -1: none), or by mask r where there is no ``mask_rows``. Ids outside the vocabulary are passed over, and so is
+    what offsets name outside their list. Rows of ``logits`` and ``out`` may be
     strided."""
     here, code = _here("logits", logits), dtype_code(logits.dtype)
     if out.dtype is not torch.float32 or out.get_device() != here:
@@ -852,29 +853,28 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, token_offsets: torch.
         raise KernelLibraryError(f"mask_words must be [masks, words], got {list(mask_words.shape)}")
     if (token_offsets is None) != (token_ids is None):
         raise KernelLibraryError("token_offsets and token_ids go together")
+    n_biases = 0 if bias_ids is None else bias_ids.numel()
     if not (bias_offsets is None) == (bias_ids is None) == (bias_values is None) or (
-            bias_ids is not None and bias_ids.numel() != bias_values.numel()):
+            bias_ids is not None and n_biases != bias_values.numel()):
         raise KernelLibraryError("bias_offsets, bias_ids and bias_values go together, a value an id")
     if mask_words is None and mask_rows is not None or mask_words is not None and mask_rows is None and mask_words.shape[0] != n_rows:
         raise KernelLibraryError("mask_rows says which of mask_words' rows a row of scores goes by; without it there is one each")
     if n_rows == 0:
         return
-    first, last = logits.data_ptr(), logits.data_ptr() + ((n_rows - 1) * logits.stride(0) + vocab) * logits.element_size()
-    if first < out.data_ptr() + ((n_rows - 1) * out.stride(0) + vocab) * 4 and out.data_ptr() < last:
+    first, to, from_stride, stride = logits.data_ptr(), out.data_ptr(), logits.stride(0), out.stride(0)
+    if first < to + ((n_rows - 1) * stride + vocab) * 4 and to < first + ((n_rows - 1) * from_stride + vocab) * logits.element_size():
         # the same rows, or other columns of the same buffer
-        stride = out.stride(0)
-        apart = (out.data_ptr() - first) // 4 % max(stride, 1)
-        if code != F32 or n_rows > 1 and stride != logits.stride(0) or not (
-                out.data_ptr() == first or n_rows > 1 and vocab <= apart <= stride - vocab):
+        apart = (to - first) // 4 % max(stride, 1)
+        if code != F32 or n_rows > 1 and stride != from_stride or not (to == first or n_rows > 1 and vocab <= apart <= stride - vocab):
             raise KernelLibraryError("out lies over a part of logits; it may be the same rows, or others")
+    n_masks, mask_width = (0, 0) if mask_words is None else mask_words.shape
     n_ids = 0 if token_ids is None else token_ids.numel()
     need = _adjust_logits_scratch(n_ids, n_rows, vocab)
     scratch = torch.empty(need // 4, dtype=torch.int32, device=logits.device) if need else None
     check(library().mx_adjust_logits(
-        _ptr(logits), code, logits.stride(0), _ptr(out), out.stride(0), n_rows, vocab, _ptr(token_offsets), _ptr(token_ids), n_ids,
+        first, code, from_stride, to, stride, n_rows, vocab, _ptr(token_offsets), _ptr(token_ids), n_ids,
         _ptr(repeat_penalty), _ptr(presence_penalty), _ptr(frequency_penalty), _ptr(bias_offsets), _ptr(bias_ids), _ptr(bias_values),
-        _ptr(mask_words), 0 if mask_words is None else mask_words.shape[0], 0 if mask_words is None else mask_words.shape[1],
-        _ptr(mask_rows), _ptr(pending_ids), _ptr(scratch), _stream()), "adjust_logits")
+        n_biases, _ptr(mask_words), n_masks, mask_width, _ptr(mask_rows), _ptr(pending_ids), _ptr(scratch), _stream()), "adjust_logits")
     _launched(2 if need else 1)
 
 

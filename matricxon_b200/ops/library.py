@@ -60,7 +60,7 @@ _SIGNATURES: dict[str, tuple[list, object]] = {
     "mx_paged_attention_shared": ([P, I, I, P, L, I, P, I, P, P, P, P, P, P, I, I, I, I, I, I, I, F, F, P, P, I, I, I, I, I, P, P, P], I),
     "mx_step_tables": ([P, P, P, I, P, I, I, P, I, P, I, L, P, P, I, I, P, P, P, P, I, P, P, P, P], I),
     "mx_adjust_logits_scratch": ([L, I, I], L),
-    "mx_adjust_logits": ([P, I, L, P, L, I, I, P, P, L, P, P, P, P, P, P, P, I, I, P, P, P, P], I),
+    "mx_adjust_logits": ([P, I, L, P, L, I, I, P, P, L, P, P, P, P, P, P, L, P, I, I, P, P, P, P], I),
     "mx_rmsnorm": ([P, P, P, F, P, I, I, I, F, L, P], I),
     "mx_add_row": ([P, P, I, I, P], I),
     "mx_rmsnorm_pending": ([P, P, P, I, P, P, F, P, I, I, I, F, P], I),

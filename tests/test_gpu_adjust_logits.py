@@ -259,3 +259,51 @@ def test_refusals():
         adjust(buffer[:300].view(3, 100), buffer[4:304].view(3, 100))
     with pytest.raises(KernelLibraryError):                 # rows that lie in one another
         adjust(logits, out[:1].expand(3, 100))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,tokens", [(3, 20001, 8000), (5, 9000, 3000), (37, 70001, 4500), (37, 70001, 60), (2, 40000, 30000)])
+def test_lists_over_several_stretches(rows, vocab, tokens, dtype):
+    """Ids dealt out to ten stretches of a turn and to nine of four turns, and lists short enough not to be."""
+    case = Case(rows, vocab, tokens=tokens, biases=40, dtype=dtype, seed=rows)
+    case.check(adjust(case.logits.to(DEV), torch.empty(rows, vocab, device=DEV), **case.device()))
+
+
+@pytest.mark.parametrize("rows,vocab,tokens", [(4, 700, 60), (4, 20001, 8000)])
+@pytest.mark.parametrize("which", ["token", "bias"])
+@pytest.mark.parametrize("bad", [(-5, 10, 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1), (0, 70, 30, 90, 100), (2 ** 31 - 1, 0, -2 ** 31, 50, 20),
+                                 (90, 60, 40, 20, 0), (0, 10 ** 6, 10 ** 6 + 1, 10 ** 6 + 2, 10 ** 6 + 3), (100, 100, 100, 100, 10 ** 6)], ids=str)
+def test_offsets_outside_their_list(rows, vocab, tokens, which, bad):
+    """A row takes what lies inside the list, whether ids are dealt out first or not; parts may overlap."""
+    case = Case(rows, vocab, tokens=tokens, biases=90, seed=3)
+    args = case.device()
+    lists = {"token": [v for row in case.tokens for v in row], "bias": [pair for row in case.biases for pair in row]}
+    size = len(lists[which])
+    scale = max(1, size // 100)
+    bad = [o if abs(o) > 1000 else o * scale for o in bad]
+    inside = [min(max(o, 0), size) for o in bad]
+    parts = [lists[which][a:b] for a, b in zip(inside, inside[1:])]
+    if which == "token":
+        case.tokens = parts
+    else:
+        case.biases = parts
+    args[f"{which}_offsets"].copy_(ints(bad))
+    out = torch.empty(rows, vocab, device=DEV)
+    for _ in range(3):
+        case.check(adjust(case.logits.to(DEV), out.fill_(float("nan")), **args))
+
+
+def test_captured_with_offsets_that_fall_and_rise_again():
+    case = Case(4, 20001, tokens=8000, seed=6)
+    args, logits, out = case.device(), case.logits.to(DEV), torch.empty(4, 20001, device=DEV)
+    adjust(logits, out, **args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        adjust(logits, out, **args)
+    ids = [v for row in case.tokens for v in row]
+    for offsets in ([0, 9000, 3000, 12000, 10], [0, 50, 8000, 8000, len(ids)], [5, 4, 3, 2, 1 << 30]):
+        args["token_offsets"].copy_(ints(offsets))
+        graph.replay()
+        case.tokens = [ids[a:b] for a, b in zip(offsets, offsets[1:])]
+        case.check(out)
