@@ -297,7 +297,7 @@ attention_mma_kernel(const MmaAttnParams p) {
     }
     const int group = p.group;
     if (KEYS != SHARED_KEYS) {
-        q_start = p.cu_q[seq];
+        q_start = KEYS == OWN_KEYS ? max(p.cu_q[seq], 0) : p.cu_q[seq];
         q_len = (KEYS == OWN_KEYS ? min(p.cu_q[seq + 1], p.shared.n_tokens) : p.cu_q[seq + 1]) - q_start;
         ctx = p.context_lens[seq];
     }

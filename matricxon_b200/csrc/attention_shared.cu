@@ -303,23 +303,42 @@ shared_simt_kernel(const SharedAttnParams p) {
     if (!SHARED) wait_for_shared_keys();
 }
 
-// The join: a warp a (token, head), four dimensions a lane. A token of no sequence is left alone.
+// The join: a warp a (token, head), four dimensions a lane. A token of no sequence is left alone. So is one whose parts nobody
+// wrote, which is reported: a token that is not its sequence's (by the sequences' starts), whose sequence is in no group, or
+// that does not fit its sequence's narrow tile; with groups whose starts fall, all are. The lists are read before the wait:
+// the kernels before this one have waited for what wrote them, and this one begins after that (from L2, where it is then).
 constexpr int JOIN_WARPS = 4;
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
 shared_join_kernel(const float* part_o, const float* part_ml, T* out, int out_stride, const int* cu_q, const float* sink,
-                   int n_heads, int head_dim, long long n_pairs, const SharedPrefixParams shared, int* status) {
+                   int n_heads, int head_dim, long long n_pairs, int tile_tokens, const SharedPrefixParams shared, int* status) {
     pdl_trigger();
     const long long pair = (long long)blockIdx.x * JOIN_WARPS + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
+    const int token = (int)(min(pair, n_pairs - 1) / n_heads), head = (int)(pair - (long long)token * n_heads);
+    const int rows = __ldcg(cu_q + shared.n_seqs), seq = __ldcg(shared.tok_seq + token);
+    bool written = seq >= 0 && seq < shared.n_seqs;
+    if (written) {
+        const int start = __ldcg(cu_q + seq), end = __ldcg(cu_q + seq + 1);
+        written = start >= 0 && token >= start && token < end && token - start < tile_tokens;
+    }
+    if (shared.n_shared_parts > 0) {
+        auto start_of = [&](int g) { return min(max(__ldcg(shared.first + g), 0), shared.n_seqs); };
+        bool rises = true;
+        for (int g = threadIdx.x; g < shared.n_groups; g += JOIN_WARPS * 32) rises = rises && start_of(g) <= start_of(g + 1);
+        written = written && seq >= start_of(0) && seq < start_of(shared.n_groups);
+        written = __syncthreads_and(rises) && written;
+    }
     pdl_wait();
     if (pair >= n_pairs) return;
     part_o = after_wait(part_o);
     part_ml = after_wait(part_ml);
-    const int token = (int)(pair / n_heads), head = (int)(pair - (long long)token * n_heads);
-    const int rows = cu_q[shared.n_seqs];
     if (rows > shared.n_tokens && pair == 0 && lane == 0) atomicOr(status, MX_STATUS_BAD_STEP);
     if (token >= rows) return;
+    if (!written) {
+        if (lane == 0) atomicOr(status, MX_STATUS_BAD_STEP);
+        return;
+    }
     const size_t base = (size_t)pair * shared.n_parts;
     float m = -INFINITY;
     for (int s = lane; s < shared.n_parts; s += 32) m = fmaxf(m, part_ml[(base + s) * 2]);
@@ -376,11 +395,11 @@ int launch_simt(const SharedAttnParams& p, unsigned n_tiles, cudaStream_t stream
 }
 
 template <typename T>
-int launch_join(const SharedAttnParams& p, T* out, int out_stride, const float* sink, cudaStream_t stream) {
+int launch_join(const SharedAttnParams& p, T* out, int out_stride, const float* sink, int tile_tokens, cudaStream_t stream) {
     const long long pairs = (long long)p.n_tokens * p.n_heads;
     const cudaError_t e = mx_launch_beside(shared_join_kernel<T>, dim3((unsigned)((pairs + JOIN_WARPS - 1) / JOIN_WARPS)),
                                            dim3(JOIN_WARPS * 32), 0, stream, (const float*)p.part_o, (const float*)p.part_ml, out, out_stride,
-                                           p.cu_q, sink, p.n_heads, p.head_dim, pairs, p.shared, p.status);
+                                           p.cu_q, sink, p.n_heads, p.head_dim, pairs, tile_tokens, p.shared, p.status);
     if (e != cudaSuccess) {
         mx_set_error("attention over shared keys: launch failed: %s", cudaGetErrorString(e));
         return (int)e;
@@ -557,6 +576,8 @@ extern "C" int mx_paged_attention_shared(const void* q, int dtype, int q_stride,
                                        : launch_simt<__nv_bfloat16, 1, false>(p, plan.own_tiles, stream);
     }
     if (rc != MX_OK) return rc;
-    if (dtype == MX_DTYPE_F32) return launch_join<float>(p, (float*)out, out_stride, sink, stream);
-    return launch_join<__nv_bfloat16>(p, (__nv_bfloat16*)out, out_stride, sink, stream);
+    // tokens of a sequence that its tile of the own keys has room for
+    const int tile_tokens = plan.narrow ? 16 / p.group : 0x7fffffff;
+    if (dtype == MX_DTYPE_F32) return launch_join<float>(p, (float*)out, out_stride, sink, tile_tokens, stream);
+    return launch_join<__nv_bfloat16>(p, (__nv_bfloat16*)out, out_stride, sink, tile_tokens, stream);
 }

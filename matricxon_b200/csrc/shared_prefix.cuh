@@ -74,7 +74,7 @@ __device__ __forceinline__ GroupTile find_group_tile(const SharedPrefixParams& p
         if (g < p.n_groups) {
             seq = min(max(p.first[g], 0), p.n_seqs);
             end = min(max(p.first[g + 1], 0), p.n_seqs);
-            start = min(cu_q[seq], p.n_tokens);
+            start = min(max(cu_q[seq], 0), p.n_tokens);
             tokens = min(cu_q[end], p.n_tokens) - start;
         }
         const int tiles = tokens > 0 ? (tokens * rows + per_tile - 1) / per_tile : 0;
@@ -143,7 +143,7 @@ __device__ __forceinline__ SequenceTile find_sequence_tile(const SharedPrefixPar
     int before = 0;
     for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
         const int s = s0 + lane;
-        const int mine = s < p.n_seqs ? max(0, min(cu_q[s + 1], p.n_tokens) - cu_q[s]) * group : 0;
+        const int mine = s < p.n_seqs ? max(0, min(cu_q[s + 1], p.n_tokens) - max(cu_q[s], 0)) * group : 0;
         const int tiles = (mine + rows - 1) / rows;
         int through = tiles;
 #pragma unroll

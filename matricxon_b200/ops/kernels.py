@@ -715,9 +715,12 @@ def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, 
     through the first other one that does. A page that the shared keys fill in part is the first sequence's alone and has to
     be in its table while any sequence sees those keys (otherwise the status word is set). ``q``, ``out``, ``window``, ``softcap`` and ``sink`` as in ``paged_attention``;
     sequence s brings rows ``cu_q[s] .. cu_q[s + 1] - 1``, row i of it at position ``context_lens[s] + i``, which
-    ``positions`` and ``tok_seq`` repeat row by row. Rows from ``cu_q[-1]`` on are left alone.
+    ``positions`` and ``tok_seq`` repeat row by row. Rows from ``cu_q[-1]`` on are left alone. So are rows whose ``tok_seq`` is
+    not their sequence, and rows of sequences that no group holds; they set the status word (sequences without tokens need no
+    group).
 
-    ``max_q_len``: no sequence brings more tokens, and all together at most ``n_tokens`` (otherwise the status word is set). ``max_shared_len``,
+    ``max_q_len``: no sequence brings more tokens, and all together at most ``n_tokens`` (otherwise the status word is set, and
+    what does not fit is left out). ``max_shared_len``,
     ``max_own_len`` (keys that a sequence shares, and does not) are for sizing: with other numbers the result is the same
     up to rounding. All three are host numbers, so that a captured step can be replayed with other lengths and groups
     below them. ``scratch`` (float32) is taken from torch's allocator where none is given. The shared keys and values have to be

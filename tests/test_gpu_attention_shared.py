@@ -437,3 +437,65 @@ def forget_tails(step):
 def test_slots_before_a_sequences_own_keys_hold_anything(shape, masks, groups):
     step = forget_tails(Step(groups, *shape, seed=11))
     close(step, step.run(**masks), **masks)
+
+
+@pytest.mark.parametrize("shape", [SHAPES[0], SHAPES[5], SHAPES[10]], ids=str)
+@pytest.mark.parametrize("first,lost", [([0, 2], (2, 3)), ([1, 4], (0,)), ([0, 1, 3], (3,)), ([0, 3, 1, 4], (0, 1, 2, 3)), ([2, 2], (0, 1, 2, 3)),
+                                        ([0, 2, 9], ()), ([-3, 2, 4], ())], ids=str)
+def test_sequences_of_no_group_are_reported_and_left_alone(shape, first, lost):
+    """Lists of groups that leave sequences out, or whose starts fall: rows of such sequences stay, the status word is set,
+    whatever the scratch memory holds. Starts outside the sequences are taken for their ends, as ever."""
+    step = Step([(64, [(30, 1), (9, 2), (0, 1), (5, 1)])], *shape, seed=3)
+    whole = step.run().clone()
+    assert step.d["status"].item() == 0
+    step.d["first"] = ints(first)
+    out = step.run(scratch=torch.full((1 << 22,), 1e6, device=DEV))
+    assert step.d["status"].item() == (16 if lost else 0)
+    seq = step.d["tok_seq"].tolist()
+    ref, bound = step.plain()
+    for row, s in enumerate(seq):
+        if s in lost:
+            assert torch.isnan(out[row]).all()
+        else:
+            assert ((out[row].double().cpu() - ref[row]).abs() <= bound[row]).all()
+    assert not torch.isnan(whole).any()
+
+
+@pytest.mark.parametrize("shape", [SHAPES[0], SHAPES[5], SHAPES[10]], ids=str)
+def test_sequences_without_tokens_may_be_of_no_group(shape):
+    """The padding of a batch of a fixed size, behind the groups or before them."""
+    step = Step([(64, [(30, 1), (9, 1), (0, 0), (5, 0)])], *shape, seed=3)
+    step.d["first"] = ints([0, 2])
+    close(step, step.run())
+    step = Step([(64, [(30, 0), (9, 1), (0, 1)])], *shape, seed=3)
+    step.d["first"] = ints([1, 3])
+    step.d["tables"][1, :4] = step.d["tables"][0, :4]
+    close(step, step.run())
+
+
+@pytest.mark.parametrize("shape", [SHAPES[0], SHAPES[5], SHAPES[10]], ids=str)
+def test_rows_with_another_sequences_number_are_reported_and_left_alone(shape):
+    step = Step([(64, [(30, 1), (9, 1), (0, 1)])], *shape, seed=3)
+    step.d["tok_seq"] = ints([0, -1, 0])
+    out = step.run(scratch=torch.full((1 << 22,), 1e6, device=DEV))
+    assert step.d["status"].item() == 16
+    ref, bound = step.plain()
+    assert ((out[0].double().cpu() - ref[0]).abs() <= bound[0]).all() and torch.isnan(out[1:]).all()
+
+
+def test_tokens_beyond_what_was_said_are_left_alone():
+    """Two of a sequence's nine tokens fit the sixteen rows of its tile."""
+    step = Step([(64, [(30, 1), (30, 9)])], 16, 2, 128, 16, BF16, seed=3)
+    out = step.run(max_q_len=2, scratch=torch.full((1 << 22,), 1e6, device=DEV))
+    assert step.d["status"].item() == 16
+    ref, bound = step.plain()
+    assert ((out[:3].double().cpu() - ref[:3]).abs() <= bound[:3]).all() and torch.isnan(out[3:]).all()
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_results_do_not_hang_on_the_scratch_memory(shape):
+    for name in ("groups", "portions"):
+        step = Step(STEPS[name], *shape, seed=4)
+        outs = [step.run(scratch=torch.full((1 << 23,), value, device=DEV)) for value in (0.0, 1e30, float("nan"))]
+        close(step, outs[0])
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
