@@ -45,6 +45,7 @@
 
 #include "common.cuh"
 #include "shared_prefix.cuh"
+#include "tensor_map.h"
 
 namespace {
 
@@ -730,23 +731,9 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     }
 }
 
-typedef CUresult (*AtEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-AtEncodeFn at_encode_fn() {
-    static AtEncodeFn fn = nullptr;
-    if (fn == nullptr) {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult query;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &query) == cudaSuccess &&
-            query == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<AtEncodeFn>(ptr);
-    }
-    return fn;
-}
 int at_make_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
                 const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
-    AtEncodeFn encode = at_encode_fn();
+    const MxEncodeTiledFn encode = mx_encode_tiled();
     if (encode == nullptr) MX_REFUSE("tcgen05 attention: the driver does not offer cuTensorMapEncodeTiled");
     const cuuint32_t elem[4] = {1, 1, 1, 1};
     const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims,

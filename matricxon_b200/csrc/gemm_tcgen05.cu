@@ -858,23 +858,6 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     }
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                  CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled_fn() {
-    static EncodeTiledFn fn = nullptr;
-    if (fn == nullptr) {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult query;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &query) == cudaSuccess &&
-            query == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(ptr);
-    }
-    return fn;
-}
-
 // A [rows, K] matrix with `ld` elements between rows, cut into boxes of box_rows x 64 bfloat16, or of another form.
 // Encoding a map costs the host a few microseconds and a step launches some hundred products, most of
 // them on the same weight matrices and the same activation buffers as the step before: maps are kept
@@ -915,7 +898,7 @@ int mx_tensor_map_form(CUtensorMap* map, const void* base, long long rows, long 
         *map = slot.map;
         return MX_OK;
     }
-    EncodeTiledFn encode = encode_tiled_fn();
+    const MxEncodeTiledFn encode = mx_encode_tiled();
     if (encode == nullptr) MX_REFUSE("tcgen05 gemm: the driver does not offer cuTensorMapEncodeTiled");
     const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
     const bool f32 = form == MX_MAP_F32_128B, narrow = form == MX_MAP_BF16_64B;

@@ -6,6 +6,7 @@
 #include <cuda.h>
 
 #include "common.cuh"
+#include "tensor_map.h"
 
 // A [rows, K] bfloat16 matrix with `ld` elements between rows, cut into boxes of box_rows x 64
 // (128-byte swizzle). Encoded once per distinct operand and kept (gemm_tcgen05.cu).

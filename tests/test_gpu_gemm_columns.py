@@ -162,3 +162,44 @@ def test_first_calls_from_several_threads():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", FIRST_CALLS, root], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+ON_A_NEW_THREAD = """
+import sys, threading
+sys.path.insert(0, sys.argv[1])
+sys.path.insert(0, sys.argv[1] + "/tests")
+import torch
+from test_gpu_attention_shared import SHAPES, STEPS, Step
+from matricxon_b200.ops import kernels as k
+step = Step(STEPS["groups"], *SHAPES[0], seed=2)
+scratch = torch.empty(1 << 22, device="cuda")
+out = [torch.zeros(step.n, step.heads * step.dim, dtype=step.dtype, device="cuda") for _ in range(3)]
+a, w = torch.randn(300, 512, device="cuda").bfloat16(), torch.randn(1024, 512, device="cuda").bfloat16()
+products = [torch.zeros(300, 1024, device="cuda") for _ in range(2)]
+step.run(out=out[0], scratch=scratch)
+k.gemm_columns(a, w, None, None, products[0], k.EPILOGUE_F32)
+torch.cuda.synchronize()
+failed = []
+def call(what):
+    try:
+        what()
+    except Exception as error:
+        failed.append(error)
+again = a.clone(), w.clone()                        # operands that no map was made for yet
+torch.cuda.synchronize()
+for what in (lambda: step.run(out=out[1], scratch=scratch), lambda: k.gemm_columns(*again, None, None, products[1], k.EPILOGUE_F32),
+             lambda: step.run(out=out[2], scratch=scratch)):
+    thread = threading.Thread(target=call, args=(what,))
+    thread.start()
+    thread.join()
+torch.cuda.synchronize()
+assert not failed, failed
+assert torch.equal(out[0], out[1]) and torch.equal(out[0], out[2]) and torch.equal(products[0], products[1])
+"""
+
+
+def test_calls_on_new_threads():
+    """A thread whose first use of the GPU is a call that makes tensor maps, after another thread has made some."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", ON_A_NEW_THREAD, root], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
