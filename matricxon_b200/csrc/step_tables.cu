@@ -15,7 +15,9 @@
 // changed (lengths, free pages), so a step can be laid out twice.
 //
 // Every block adds up all sequences' lengths for itself (a sequence a thread, 8 to 20 bytes each out of L2), which spares a
-// second launch or a wait between blocks; it then lays out its few sequences. A step that does not fit (more rows than the
+// second launch or a wait between blocks; it then lays out its few sequences. On the way it marks each sequence's row in a bitmap:
+// where two meet, the sequences are compared one by one, and those whose row an earlier one has bring nothing, take nothing and
+// are reported. A step that does not fit (more rows than the
 // buffers hold, more pages than there are, a length out of range) sets MX_STATUS_BAD_STEP and every block leaves an empty step:
 // all -1, nothing taken, `tables` as they were.
 // The launch after this one must not begin early: attention kernels read tables and lengths before they wait for what ran
@@ -28,6 +30,7 @@ constexpr int ST_THREADS = 512;
 constexpr int ST_OWN = 64;              // sequences a block lays out, at most
 constexpr int ST_AHEAD = 8;
 constexpr int ST_SLICE = 16384;         // block-table entries of a sequence that one block writes
+constexpr int ST_MARKS = 2048;          // words of the bitmap of rows: row r is bit r / 2048 % 32 of word r % 2048
 
 struct StepTablesParams {
     const int *q_lens, *context_lens, *rows, *shared_rows, *shared_pages, *free_pages, *n_free;
@@ -67,56 +70,86 @@ __device__ __forceinline__ Sequence read_sequence(const StepTablesParams& p, int
 __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTablesParams p) {
     __shared__ long long warp_total[ST_THREADS / 32];
     __shared__ int warp_sums[3][ST_THREADS / 32];
+    __shared__ unsigned marks[ST_MARKS];
     __shared__ Sequence own[ST_OWN];
-    __shared__ int repeated[ST_OWN], own_row[ST_OWN], own_page[ST_OWN];
+    __shared__ int own_row[ST_OWN], own_page[ST_OWN];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int first = blockIdx.x * p.per_block, last = min(p.n_seqs, first + p.per_block);
+    if (p.rows)
+        for (int i = tid; i < min(p.n_rows, ST_MARKS); i += ST_THREADS) marks[i] = 0u;
     pdl_wait();
 
     // ---- what all sequences bring and take, and what those before this block's do
     long long q_all = 0;
     int q_before = 0, need_before = 0, need_all = 0;         // (before: wrong only where the step does not fit anyway)
-    bool fits = true;
-#pragma unroll 2
-    for (int s = tid; s < p.n_seqs; s += ST_THREADS) {
-        const Sequence v = read_sequence(p, s);
-        fits = fits && v.fits;
+    auto add = [&](const Sequence& v, int s) {
         q_all += v.q;
         need_all += v.need;
         if (s < first) { q_before += v.q; need_before += v.need; }
         else if (s < last) own[s - first] = v;
-    }
-    for (int i = tid; i < ST_OWN; i += ST_THREADS) repeated[i] = 0;
+    };
+    // the threads' sums; every thread gets them, and whether all of them say `fine`
+    auto add_up = [&](bool fine) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) q_all += __shfl_xor_sync(0xffffffffu, q_all, o);
-    q_before = (int)__reduce_add_sync(0xffffffffu, (unsigned)q_before);
-    need_before = (int)__reduce_add_sync(0xffffffffu, (unsigned)need_before);
-    need_all = (int)__reduce_add_sync(0xffffffffu, (unsigned)need_all);
-    if (lane == 0) {
-        warp_total[warp] = q_all;
-        warp_sums[0][warp] = q_before; warp_sums[1][warp] = need_before; warp_sums[2][warp] = need_all;
-    }
-    const bool all_fit = __syncthreads_and(fits);
-    q_all = 0;
-    q_before = need_before = need_all = 0;
+        for (int o = 16; o > 0; o >>= 1) q_all += __shfl_xor_sync(0xffffffffu, q_all, o);
+        q_before = (int)__reduce_add_sync(0xffffffffu, (unsigned)q_before);
+        need_before = (int)__reduce_add_sync(0xffffffffu, (unsigned)need_before);
+        need_all = (int)__reduce_add_sync(0xffffffffu, (unsigned)need_all);
+        if (lane == 0) {
+            warp_total[warp] = q_all;
+            warp_sums[0][warp] = q_before; warp_sums[1][warp] = need_before; warp_sums[2][warp] = need_all;
+        }
+        const bool all_fine = __syncthreads_and(fine);
+        q_all = 0;
+        q_before = need_before = need_all = 0;
 #pragma unroll
-    for (int w = 0; w < ST_THREADS / 32; ++w) {
-        q_all += warp_total[w];
-        q_before += warp_sums[0][w]; need_before += warp_sums[1][w]; need_all += warp_sums[2][w];
+        for (int w = 0; w < ST_THREADS / 32; ++w) {
+            q_all += warp_total[w];
+            q_before += warp_sums[0][w]; need_before += warp_sums[1][w]; need_all += warp_sums[2][w];
+        }
+        return all_fine;
+    };
+    bool fits = true, met = false;
+    Sequence next = {};
+    if (tid < p.n_seqs) next = read_sequence(p, tid);
+    __syncthreads();                                         // the bitmap is empty
+    for (int s = tid; s < p.n_seqs; s += ST_THREADS) {
+        const Sequence v = next;
+        if (s + ST_THREADS < p.n_seqs) next = read_sequence(p, s + ST_THREADS);
+        fits = fits && v.fits;
+        add(v, s);
+        if (p.rows && v.row >= 0) {
+            const unsigned bit = 1u << (v.row / ST_MARKS & 31);
+            met = met || (atomicOr(&marks[v.row % ST_MARKS], bit) & bit) != 0;
+        }
+    }
+    bool all_fit = add_up(fits && !met);
+    if (!all_fit) {
+        // Something is wrong, or two rows met in a bit. `fits` goes on alone; a row that an earlier sequence has already (a warp
+        // reads the rows before its sequences together, a place for all lanes) makes the later one one of nothing.
+        __syncthreads();                                     // everybody has read the sums
+        q_all = 0;
+        q_before = need_before = need_all = 0;
+        bool none_again = true;
+        for (int s = tid; s < p.n_seqs; s += ST_THREADS) {
+            Sequence v = read_sequence(p, s);
+            bool again = false;
+            if (p.rows && v.row >= 0)
+                for (int earlier = 0; earlier < s; ++earlier) again = again || p.rows[earlier] == v.row;
+            if (again) {
+                v.q = v.context = v.shared = v.have = v.need = v.seen_from = 0;
+                v.row = v.shared_row = -1;
+                none_again = false;
+            }
+            add(v, s);
+        }
+        none_again = add_up(none_again);
+        all_fit = __syncthreads_and(fits);
+        if (!none_again && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) atomicOr(p.status, MX_STATUS_BAD_STEP);
     }
     const int n_free = min(*p.n_free, p.n_free_most);
     const bool possible = all_fit && q_all <= p.n_tokens && need_all <= n_free;
     const int total = possible ? (int)q_all : 0;
-    // a row that an earlier sequence has already: the later one is laid out as empty
-    if (possible && p.rows) {
-        for (int s = tid; s < last; s += ST_THREADS) {
-            const int row = p.rows[s];
-            if (row < 0) continue;
-            for (int i = max(first, s + 1); i < last; ++i)
-                if (own[i - first].row == row) repeated[i - first] = 1;
-        }
-        __syncthreads();
-    }
     if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) {
         p.cu_q[0] = 0;
         *p.taken = possible ? need_all : 0;
@@ -130,10 +163,7 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTable
         for (int i = 0; i < tid; ++i) { rows_before += own[i].q; pages_before += own[i].need; }
         own_row[tid] = rows_before;
         own_page[tid] = pages_before;
-        if (blockIdx.y == 0) {
-            p.cu_q[first + tid + 1] = possible ? rows_before + own[tid].q : 0;
-            if (possible && repeated[tid]) atomicOr(p.status, MX_STATUS_BAD_STEP);
-        }
+        if (blockIdx.y == 0) p.cu_q[first + tid + 1] = possible ? rows_before + own[tid].q : 0;
     }
     __syncthreads();
     // pages that nobody sees any more lie between the kept ones and the first that the next query needs
@@ -142,7 +172,7 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTable
     bool bad_page = false;
     for (int i = 0; i < mine_n; ++i) {
         const Sequence v = own[i];
-        const bool there = possible && v.row >= 0 && !repeated[i];
+        const bool there = possible && v.row >= 0;
         const int end = there ? min(k_end, v.have + v.need) : 0;
         int* out = p.block_tables + (size_t)(first + i) * p.width;
         int* row = p.tables + (size_t)max(v.row, 0) * p.width;
@@ -176,18 +206,15 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTable
         // their token rows, a warp a sequence of few (decoding requests), the block one of more
         auto token_rows = [&](int i, int r0, int step) {
             const Sequence& v = own[i];
-            const bool there = !repeated[i];
             for (int r = r0; r < v.q; r += step) {
                 const int position = v.context + r, k = (int)((unsigned)position / (unsigned)p.page_size);
                 int slot = -1;
-                if (there) {
-                    const int page = k >= v.have ? p.free_pages[own_page[i] + k - v.have] : p.tables[(size_t)v.row * p.width + k];
-                    if (page >= 0 && page < p.n_pages) slot = page * p.page_size + position - k * p.page_size;
-                    else bad_page = true;
-                }
+                const int page = k >= v.have ? p.free_pages[own_page[i] + k - v.have] : p.tables[(size_t)v.row * p.width + k];
+                if (page >= 0 && page < p.n_pages) slot = page * p.page_size + position - k * p.page_size;
+                else bad_page = true;
                 const int t = own_row[i] + r;
-                p.positions[t] = there ? position : 0;
-                p.tok_seq[t] = there ? first + i : -1;
+                p.positions[t] = position;
+                p.tok_seq[t] = first + i;
                 p.slots[t] = slot;
             }
         };

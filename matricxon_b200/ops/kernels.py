@@ -790,7 +790,8 @@ def step_tables(q_lens: torch.Tensor, context_lens: torch.Tensor, rows: torch.Te
     token: 0, -1, -1) and ``block_tables`` [sequences, width], -1 where there is no page or none that a query from
     ``context_lens[s]`` on sees: ``window`` and ``keep_first`` as in ``paged_attention``, a negative window for blocks. Lengths and
     free pages are only read, so the same step may be laid out again. A step that does not fit sets the status word and
-    comes out empty, with ``tables`` as they were; of two sequences with one row the later one does."""
+    comes out empty, with ``tables`` as they were. Of two sequences with one row the later one brings no rows and takes no pages,
+    and the status word is set."""
     here = _here("q_lens", q_lens)
     n_seqs, n_tokens = q_lens.numel(), positions.numel()
     if tables.ndim != 2:

@@ -282,3 +282,50 @@ def test_refusals():
     case.page, case.n_pages = 1 << 16, 1 << 16
     with pytest.raises(KernelLibraryError):
         case.run()
+
+
+@pytest.mark.parametrize("n", [4, 70, 700])
+@pytest.mark.parametrize("n_rows", [None, 70000])
+def test_a_row_listed_twice_takes_nothing(n, n_rows):
+    """The later sequences of a row bring no rows and take no pages; the others come out as without them."""
+    rng = random.Random(n)
+    case = Case([rng.choice((1, 1, 17)) for _ in range(n)], [16 * rng.randrange(4) for _ in range(n)], 16, seed=n, spare=40 * n)
+    if n_rows:                                            # rows far apart
+        case.rows = [r * (n_rows // len(case.tables)) for r in case.rows]
+        tables = [[-1] * case.width for _ in range(n_rows)]
+        for s, row in enumerate(case.rows):
+            for k in range(-(-case.context[s] // 16)):
+                tables[row][k] = s * 4 + k
+        case.tables, case.n_pages = tables, 4 * n + n * 2
+        case.free = list(range(4 * n, 6 * n))
+    again = sorted(rng.sample(range(1, n), max(1, n // 9)))
+    without = list(case.q)
+    for s in again:
+        without[s] = 0
+    case.device()
+    for s in again:
+        case.inputs["rows"][s] = case.rows[rng.choice([0] + [r for r in range(s) if r not in again])]
+    got = case.run()
+    assert case.status.item() == 16
+    case.q = without
+    expected = case.expected()
+    for s in again:
+        expected["block_tables"][s] = [-1] * case.width
+    assert got == expected
+    case.status.zero_()
+    assert case.run() == expected and case.status.item() == 16
+
+
+def test_rows_far_apart_that_are_not_the_same():
+    """Rows 65,536 apart, which the kernel cannot tell apart at first."""
+    rows = [5, 5 + 65536, 9, 131081, 70000, 65545]
+    case = Case([1, 2, 1, 17, 1, 1], [5, 40, 16, 0, 31, 100], 16, seed=1)
+    case.rows = rows
+    tables = [[-1] * case.width for _ in range(131100)]
+    at = 0
+    for s, row in enumerate(rows):
+        for k in range(-(-case.context[s] // 16)):
+            tables[row][k], at = at, at + 1
+    case.tables, case.free, case.n_pages = tables, list(range(at, at + 20)), at + 20
+    case.device()
+    assert case.run() == case.expected() and case.status.item() == 0
