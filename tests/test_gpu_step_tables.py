@@ -329,3 +329,52 @@ def test_rows_far_apart_that_are_not_the_same():
     case.tables, case.free, case.n_pages = tables, list(range(at, at + 20)), at + 20
     case.device()
     assert case.run() == case.expected() and case.status.item() == 0
+
+
+def stale(case, seed):
+    """Valid page numbers of an earlier tenant behind what each row holds."""
+    rng = random.Random(seed)
+    for s, row in enumerate(case.rows):
+        for k in range(-(-case.context[s] // case.page), case.width):
+            case.tables[row][k] = rng.randrange(case.n_pages)
+    return case
+
+
+@pytest.mark.parametrize("n", [3, 40, 700])
+@pytest.mark.parametrize("use_rows", [True, False])
+def test_shared_pages_that_the_leader_takes_in_the_same_step(n, use_rows):
+    """A prompt portion fills the prefix's pages in the step in which others begin behind them."""
+    rng = random.Random(n)
+    lead = n // 2
+    context = [160 + rng.randrange(40) for _ in range(n)]
+    q = [rng.choice((1, 1, 9)) for _ in range(n)]
+    context[lead], q[lead] = 40, 130
+    shared = [(lead, rng.randrange(1, 11)) if s != lead and rng.random() < 0.8 else (-1, 0) for s in range(n)]
+    shared[0], shared[-1] = (lead, 10), (lead, 7)
+    if lead in (0, n - 1):
+        shared[lead] = (-1, 0)
+    case = stale(Case(q, context, 16, seed=n, shared=shared, use_rows=use_rows), n).device()
+    expected = case.expected()
+    for _ in range(5):
+        assert case.run() == expected
+        assert case.status.item() == 0
+
+
+def test_more_shared_pages_than_the_leader_has():
+    """Pages that the leader neither holds nor takes are none, and reported, whatever stands in its row."""
+    case = stale(Case([1, 3, 1], [200, 20, 200], 16, seed=4, shared=[(1, 2), (-1, 0), (1, 5)]), 4).device()
+    expected = case.expected()
+    expected["block_tables"][2][2:5] = [-1] * 3
+    assert case.run() == expected and case.status.item() == 4
+
+
+def test_a_leader_that_is_listed_twice():
+    """The first sequence of a row is the leader, and what the later ones would take is not counted before it."""
+    case = stale(Case([5, 17, 20, 1], [16, 30, 30, 90], 16, seed=4, shared=[(-1, 0), (-1, 0), (-1, 0), (2, 3)]), 4).device()
+    case.inputs["rows"][1] = case.rows[0]
+    got = case.run()
+    assert case.status.item() == 16
+    case.q[1] = 0
+    expected = case.expected()
+    expected["block_tables"][1] = [-1] * case.width
+    assert got == expected
