@@ -14,9 +14,11 @@ are applied in that order after the repeat penalty and before everything else, g
 
 from __future__ import annotations
 
-import math
 from collections.abc import Mapping
 from dataclasses import dataclass
+
+
+LARGEST_FLOAT32 = (2.0 - 2.0 ** -23) * 2.0 ** 127
 
 
 @dataclass(frozen=True)
@@ -37,10 +39,11 @@ class SamplingConfig:
         pairs = self.logit_bias.items() if isinstance(self.logit_bias, Mapping) else (self.logit_bias or ())
         # a token named twice keeps its later bias
         bias = tuple({int(token): float(value) for token, value in pairs}.items())
-        if not all(math.isfinite(value) for _, value in bias):
-            raise ValueError("a logit_bias must be finite; allowed_token_ids rules tokens out")
-        if not (math.isfinite(self.presence_penalty) and math.isfinite(self.frequency_penalty)):
-            raise ValueError("presence_penalty and frequency_penalty must be finite")
+        # scores are 32-bit numbers: what is beyond their range would become infinite there (nan fails the comparisons too)
+        if not all(abs(value) <= LARGEST_FLOAT32 for _, value in bias):
+            raise ValueError("a logit_bias must be finite as a 32-bit number; allowed_token_ids rules tokens out")
+        if not (abs(self.presence_penalty) <= LARGEST_FLOAT32 and abs(self.frequency_penalty) <= LARGEST_FLOAT32):
+            raise ValueError("presence_penalty and frequency_penalty must be finite as 32-bit numbers")
         allowed = self.allowed_token_ids
         if allowed is not None:
             allowed = tuple(sorted({int(token) for token in allowed}))

@@ -49,3 +49,16 @@ def test_who_penalises_repeats():
         for token in (4, 4, 7):
             sampler.accept(token)
     assert plain.penalty_ids() == [4, 7] and adjusted.penalty_ids() == []
+
+
+@pytest.mark.parametrize("value", [1e39, -1e39, 3.5e38, -3.5e38, 1e308])
+@pytest.mark.parametrize("name", ["logit_bias", "presence_penalty", "frequency_penalty"])
+def test_numbers_beyond_the_scores_32_bits_are_refused(name, value):
+    with pytest.raises(ValueError, match="32-bit"):
+        SamplingConfig(**{name: {3: value} if name == "logit_bias" else value})
+
+
+@pytest.mark.parametrize("value", [3.4e38, -3.4e38, float(np.finfo(np.float32).max), 1e-50])
+def test_numbers_within_them_stay_finite(value):
+    config = SamplingConfig(logit_bias={3: value}, presence_penalty=value, frequency_penalty=value)
+    assert np.isfinite(np.asarray([config.logit_bias[0][1], config.presence_penalty, config.frequency_penalty], dtype=np.float32)).all()
