@@ -804,17 +804,18 @@ def step_tables(q_lens: torch.Tensor, context_lens: torch.Tensor, rows: torch.Te
               ("tok_seq", tok_seq, n_tokens), ("cu_q", cu_q, n_seqs + 1), ("slots", slots, n_tokens),
               ("block_tables", block_tables, n_seqs * width), ("taken", taken, -1), ("status", status, -1),
               ("shared_rows", shared_rows, n_seqs), ("shared_pages", shared_pages, n_seqs))
-    if block_tables.data_ptr() == tables.data_ptr():
+    step, kept = block_tables.data_ptr(), tables.data_ptr()
+    if step < kept + 4 * tables.numel() and kept < step + 4 * n_seqs * width:
         raise KernelLibraryError("block_tables are the step's own: tables hold what the requests keep")
     if n_free.numel() < 1 or taken.numel() < 1 or status.numel() < 1:
         raise KernelLibraryError("n_free, taken and status hold a number each")
     if rows is None and tables.shape[0] < n_seqs:
         raise KernelLibraryError(f"{n_seqs} sequences need as many rows of tables, got {tables.shape[0]}")
     check(library().mx_step_tables(
-        q_lens.data_ptr(), context_lens.data_ptr(), _ptr(rows), n_seqs, tables.data_ptr(), tables.shape[0], width,
+        q_lens.data_ptr(), context_lens.data_ptr(), _ptr(rows), n_seqs, kept, tables.shape[0], width,
         free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr(), int(page_size), int(n_pages), _ptr(shared_rows),
         _ptr(shared_pages), int(window or 0), int(keep_first), positions.data_ptr(), tok_seq.data_ptr(), cu_q.data_ptr(),
-        slots.data_ptr(), n_tokens, block_tables.data_ptr(), taken.data_ptr(), status.data_ptr(), _stream()), "step_tables")
+        slots.data_ptr(), n_tokens, step, taken.data_ptr(), status.data_ptr(), _stream()), "step_tables")
     _launched()
 
 

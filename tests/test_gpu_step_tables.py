@@ -378,3 +378,49 @@ def test_a_leader_that_is_listed_twice():
     expected = case.expected()
     expected["block_tables"][1] = [-1] * case.width
     assert got == expected
+
+
+def test_tables_that_lie_in_one_another_are_refused():
+    """The step's block tables in a part of the requests' tables, or over their end."""
+    from matricxon_b200.ops.library import KernelLibraryError
+
+    for begin in (1, 4, 11):
+        case = Case([1, 2], [5, 6], 16, width=3).device()
+        memory = torch.full((6 * 3 + 20,), -1, dtype=torch.int32, device=DEV)
+        memory[:18] = case.inputs["tables"].view(-1)
+        case.inputs["tables"] = memory[:18].view(6, 3)
+        case.outputs["block_tables"] = memory[begin:begin + 6].view(2, 3)
+        with pytest.raises(KernelLibraryError):
+            case.run()
+        case = Case([1, 2], [5, 6], 16, width=3).device()
+        memory[6:24] = case.inputs["tables"].view(-1)
+        case.inputs["tables"] = memory[6:24].view(6, 3)
+        case.outputs["block_tables"] = memory[1:7].view(2, 3)
+        with pytest.raises(KernelLibraryError):
+            case.run()
+    case = Case([1, 2], [5, 6], 16, width=3).device()             # side by side: fine
+    memory[:18] = case.inputs["tables"].view(-1)
+    case.inputs["tables"], case.outputs["block_tables"] = memory[:18].view(6, 3), memory[18:24].view(2, 3)
+    assert case.run() == case.expected() and case.status.item() == 0
+
+
+def test_calls_queued_on_two_streams():
+    """Calls with inputs and outputs of their own, queued on two streams without reading back in between."""
+    cases = [random_case(300, 16, s).device() for s in range(8)]
+    expected = [case.expected() for case in cases]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    from matricxon_b200.ops import kernels
+
+    for _ in range(20):
+        for i, case in enumerate(cases):
+            with torch.cuda.stream(streams[i % 2]):
+                a, o = case.inputs, case.outputs
+                for out in o.values():
+                    out.fill_(77)
+                kernels.step_tables(a["q_lens"], a["context_lens"], a["rows"], a["tables"], a["free_pages"], a["n_free"], 16, case.n_pages,
+                                    o["positions"], o["tok_seq"], o["cu_q"], o["slots"], o["block_tables"], o["taken"], case.status)
+    torch.cuda.synchronize()
+    for case, want in zip(cases, expected):
+        assert {**{k: v.tolist() for k, v in case.outputs.items()}, "tables": case.inputs["tables"].tolist()} == want
+        assert case.status.item() == 0
