@@ -751,6 +751,9 @@ def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, 
         raise KernelLibraryError(f"q must hold rows of {width} numbers, q_stride apart, got {list(q.shape)}")
     if out.ndim != 2 or out.shape[0] < n_tokens or out.shape[1] != width or out.stride(1) != 1:
         raise KernelLibraryError(f"out must hold {n_tokens} rows of {width} numbers, got {list(out.shape)}")
+    out_stride = out.stride(0)
+    if out_stride < width and n_tokens > 1 or max(out_stride, q_stride) > 0x7fffffff:
+        raise KernelLibraryError(f"rows of out must not overlap, and rows be less than 2^31 numbers apart, got strides {q_stride}, {out_stride}")
     if n_tokens <= 0 or n_seqs == 0:
         return
     aligned = q_stride % 8 == 0 and q.data_ptr() % 16 == 0 and cache.data_ptr() % 16 == 0
@@ -767,7 +770,7 @@ def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, 
         q.data_ptr(), code, q_stride, cache.data_ptr(), n_pages, page_size, block_tables.data_ptr(), block_tables.shape[1],
         cu_q.data_ptr(), context_lens.data_ptr(), tok_seq.data_ptr(), positions.data_ptr(), shared_first.data_ptr(),
         shared_lens.data_ptr(), n_seqs, n_groups, n_tokens, n_heads, n_kv_heads, head_dim, int(window or 0), float(scale), float(softcap or 0.0),
-        _sink_ptr(sink, n_heads), out.data_ptr(), out.stride(0), int(max_q_len), int(max_shared_len), int(max_own_len), n_sm,
+        _sink_ptr(sink, n_heads), out.data_ptr(), out_stride, int(max_q_len), int(max_shared_len), int(max_own_len), n_sm,
         scratch.data_ptr(), status.data_ptr(), _stream()), "paged_attention_shared")
     _launched(3 if max_shared_len > 0 else 2)
 

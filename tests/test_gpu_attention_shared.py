@@ -499,3 +499,22 @@ def test_results_do_not_hang_on_the_scratch_memory(shape):
         outs = [step.run(scratch=torch.full((1 << 23,), value, device=DEV)) for value in (0.0, 1e30, float("nan"))]
         close(step, outs[0])
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_rows_that_lie_in_one_another_or_too_far_apart_are_refused():
+    from matricxon_b200.ops.library import KernelLibraryError
+
+    step = Step(STEPS["decoding"], *SHAPES[0])
+    width = step.heads * step.dim
+    with pytest.raises(KernelLibraryError):
+        step.run(out=torch.zeros(1, width, dtype=BF16, device=DEV).expand(step.n, width))
+    with pytest.raises(KernelLibraryError):
+        step.run(out=torch.zeros(step.n * width, dtype=BF16, device=DEV).as_strided((step.n, width), (width - 16, 1)))
+    one = Step(STEPS["one token"], *SHAPES[0])
+    one.d["q"] = one.d["q"].as_strided((1, width), (1 << 31, 1))       # strides are 32-bit numbers further down
+    with pytest.raises(KernelLibraryError):
+        one.run()
+    one = Step(STEPS["one token"], *SHAPES[0])
+    with pytest.raises(KernelLibraryError):
+        one.run(out=torch.zeros(width, dtype=BF16, device=DEV).as_strided((1, width), (1 << 31, 1)))
+    close(one, one.run(out=torch.zeros(width, dtype=BF16, device=DEV).as_strided((1, width), (1, 1))))     # one row lies in no other
