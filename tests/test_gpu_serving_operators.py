@@ -248,7 +248,8 @@ def test_two_streams_at_once():
 @pytest.mark.parametrize("chained", [False, True])
 @pytest.mark.parametrize("heads,kv_heads,dim,page,dtype,window", [(8, 2, 128, 16, torch.bfloat16, 64), (8, 2, 128, 16, torch.bfloat16, -96),
                                                                   (16, 4, 64, 8, torch.bfloat16, 40), (6, 2, 80, 16, torch.bfloat16, 64),
-                                                                  (24, 2, 128, 16, torch.float32, 50)])
+                                                                  (24, 2, 128, 16, torch.float32, 50), (8, 2, 128, 16, torch.bfloat16, 0),
+                                                                  (24, 2, 128, 16, torch.float32, 0)])
 def test_a_decoding_loop_under_a_window(chained, heads, kv_heads, dim, page, dtype, window):
     """Requests on one prefix, the longest first: attention on the tables that the step's kernel writes, which leave out what a
     request no longer sees. Against one softmax over each request's keys, in 64 bits, by its bounds."""
@@ -321,7 +322,7 @@ def test_a_decoding_loop_under_a_window(chained, heads, kv_heads, dim, page, dty
         graph.replay()
         for s in range(n):
             position = context[s] + i
-            low = max(0, position - window + 1) if window > 0 else position - position % -window
+            low = 0 if window == 0 else max(0, position - window + 1) if window > 0 else position - position % -window
             k, v = (t[low:position + 1].double() for t in history[s])
             rows = q[s].double().view(kv_heads, heads // kv_heads, dim)
             weights = torch.softmax(torch.einsum("kgd,jkd->kgj", rows, k) * dim ** -0.5, -1)
@@ -336,3 +337,33 @@ def test_a_decoding_loop_under_a_window(chained, heads, kv_heads, dim, page, dty
             assert block_tables[s, :low // page].max().item() < 0 if low >= page else True
     assert status.item() == 0
     assert taken_all.item() == sum(-(-(c + steps) // page) - -(-c // page) for c in context)
+
+
+@pytest.mark.parametrize("look_ahead", [True, False])
+def test_engine_penalties_change_what_is_chosen(look_ahead):
+    """Greedy requests whose plain text repeats itself: with a penalty above every score no token comes twice, with a bonus the
+    first one comes again and again, and a bias of its own size takes its token out."""
+    from test_gpu_generation import random_ids, tiny_config, tiny_tensors
+
+    from matricxon_b200 import ChatEngine, GenerationRequest, SamplingConfig
+    from matricxon_b200.engine.core import model_from_tensors
+
+    model = model_from_tensors(tiny_config("A"), tiny_tensors("A", torch.float32), dtype="float32", device=DEV)
+    vocab = model.spec.vocab_size
+    engine = ChatEngine(model, max_cache_tokens=4096, max_active=8, prefill_chunk=32, max_model_len=128, look_ahead=look_ahead)
+
+    def generate(prompts, **options):
+        config = SamplingConfig(temperature=0.0, repeat_penalty=1.0, num_predict=24, num_ctx=128, **options)
+        return [r.token_ids for r in engine.generate_batch([GenerationRequest(p, config) for p in prompts])]
+
+    prompts = [random_ids(7 + i, vocab, seed=i) for i in range(8)]
+    plain = generate(prompts)
+    prompts, plain = zip(*[(p, t) for p, t in zip(prompts, plain) if len(t) == 24 and len(set(t)) < 20])
+    assert prompts                                        # the plain choice repeats itself, or this shows nothing
+    for options in ({"frequency_penalty": 1e4}, {"presence_penalty": 1e4}):
+        for text, before in zip(generate(prompts, **options), plain):
+            assert text[0] == before[0] and len(text) == 24 and len(set(text)) == 24
+    for text, before in zip(generate(prompts, frequency_penalty=-1e4), plain):
+        assert text == [before[0]] * len(text)
+    for prompt, before in zip(prompts, plain):
+        assert before[0] not in generate([prompt], logit_bias={before[0]: -1e4})[0]
