@@ -424,3 +424,16 @@ def test_calls_queued_on_two_streams():
     for case, want in zip(cases, expected):
         assert {**{k: v.tolist() for k, v in case.outputs.items()}, "tables": case.inputs["tables"].tolist()} == want
         assert case.status.item() == 0
+
+
+def test_leaders_among_many_rows():
+    """More rows of tables than the kernel keeps notes of."""
+    shared = [(2, 10), (2, 7), (-1, 0), (4, 9), (-1, 0), (1, 12)]
+    case = Case([1, 1, 130, 3, 1, 1], [160, 200, 40, 171, 300, 200], 16, seed=5, shared=shared)
+    rows = [r * 900 for r in case.rows]
+    tables = [[-1] * case.width for _ in range(10000)]
+    for old, new in zip(case.rows, rows):
+        tables[new] = case.tables[old]
+    case.rows, case.tables = rows, tables
+    case = stale(case, 5).device()
+    assert case.run() == case.expected() and case.status.item() == 0
