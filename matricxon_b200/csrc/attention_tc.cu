@@ -329,13 +329,15 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     // group's pages, which may have to be looked for, the next ones `from` there take the place of those that are done with)
     auto read_table = [&](int* table, int from) {
         const int n_table = min(n_chunks * pages_per_chunk - from, AT_TABLE);
+        bool none = false;
         for (int i = lane; i < n_table; i += 32) {
-            const int lp = logical_page(from + i);
-            table[i] = lp < p.bt_stride ? bt[lp] : -1;
+            const int lp = logical_page(from + i), page = lp < p.bt_stride ? bt[lp] : -1;
+            table[i] = page;
+            none = none || page < 0;
         }
         // (looking for pages in the loop above would have its loads wait for one another: 202 us where this takes 192, 128
         // requests on 32,768 keys)
-        if (SHARED)
+        if (SHARED && none)
             for (int i = lane; i < n_table; i += 32) {
                 const int lp = logical_page(from + i);
                 if (table[i] < 0 && (lp + 1) * p.page_size > lo_tile) table[i] = shared_page_of_others(group_pages, lp);
