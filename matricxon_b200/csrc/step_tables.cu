@@ -33,9 +33,10 @@ constexpr int ST_THREADS = 512;
 constexpr int ST_OWN = 64;              // sequences a block lays out, at most
 constexpr int ST_AHEAD = 8;
 constexpr int ST_SLICE = 16384;         // block-table entries of a sequence that one block writes
-// Notes on rows: word r says 1 + the pages held by the sequence of row r, 0 if there is none; of more rows, row r is
-// bit r / ST_MARKS % 32 of word r % ST_MARKS.
+// Notes on rows: word r says 1 + the pages held by the sequence of row r (ST_IDLE: one that brings nothing), 0 if there is none; of
+// more rows, row r is bit r / ST_MARKS % 32 of word r % ST_MARKS.
 constexpr int ST_MARKS = 4096;
+constexpr unsigned ST_IDLE = 0x7fffffffu;
 
 struct StepTablesParams {
     const int *q_lens, *context_lens, *rows, *shared_rows, *shared_pages, *free_pages, *n_free;
@@ -127,10 +128,10 @@ __device__ __noinline__ void find_leaders(const StepTablesParams& p, const Seque
     }
     __syncthreads();
     if (tid < n) {
-        leader[tid].have = own[tid].shared;                  // not in the step: its row as it is
+        leader[tid].have = own[tid].shared;                  // not in the step, or idle: its row as it is
         if (leader[tid].seq < p.n_seqs) {
             const Sequence v = read_sequence(p, leader[tid].seq);
-            leader[tid].have = min(v.have, own[tid].shared);
+            if (v.q > 0) leader[tid].have = min(v.have, own[tid].shared);
             leader[tid].need = v.need;
         }
     }
@@ -195,7 +196,7 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const __grid_co
         add_sequence(sums, v, s, first, last, own);
         if (v.row >= 0) {
             const unsigned bit = 1u << (v.row / ST_MARKS & 31);
-            const unsigned old = noted ? atomicExch(&marks[v.row], 1u + v.have) : atomicOr(&marks[v.row % ST_MARKS], bit) & bit;
+            const unsigned old = noted ? atomicExch(&marks[v.row], v.q > 0 ? 1u + v.have : ST_IDLE) : atomicOr(&marks[v.row % ST_MARKS], bit) & bit;
             met = met || old != 0u;
         }
     }

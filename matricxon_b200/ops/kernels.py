@@ -788,8 +788,8 @@ def step_tables(q_lens: torch.Tensor, context_lens: torch.Tensor, rows: torch.Te
     beyond those it holds are the next ones of ``free_pages``, in the order of the sequences, and are stored in its row;
     ``n_free`` [1] says how many of them there are, ``taken`` [1] how many the step took. Where ``shared_rows[s]`` >= 0 its first
     ``shared_pages[s]`` pages, all full, are read from that row instead, those that its sequence takes in this very step among
-    them; pages that it neither holds nor takes are none and set the status word (a row without a sequence in this step is read
-    as it is).
+    them; pages that it neither holds nor takes are none and set the status word (a row whose sequence brings nothing in this step,
+    or is not in it, is read as it is).
 
     Written: ``cu_q`` [sequences + 1], ``positions``, ``tok_seq`` and cache ``slots`` of every token row (rows behind the last
     token: 0, -1, -1) and ``block_tables`` [sequences, width], -1 where there is no page or none that a query from

@@ -437,3 +437,19 @@ def test_leaders_among_many_rows():
     case.rows, case.tables = rows, tables
     case = stale(case, 5).device()
     assert case.run() == case.expected() and case.status.item() == 0
+
+
+@pytest.mark.parametrize("n", [4, 300])
+@pytest.mark.parametrize("use_rows", [True, False])
+@pytest.mark.parametrize("n_rows", [None, 5000])
+def test_a_leader_that_brings_nothing_is_read_as_it_is(n, use_rows, n_rows):
+    """A finished request that the batch still has a place for: its lengths are 0, its row still holds the prefix."""
+    context = [0] + [80 + s % 40 for s in range(n - 1)]
+    shared = [(-1, 0)] + [(0, 1 + s % 5) for s in range(n - 1)]
+    case = Case([0] + [1] * (n - 1), context, 16, seed=n, shared=shared, use_rows=use_rows)
+    case.n_pages += 5
+    case.tables[case.rows[0]][:5] = range(case.n_pages - 5, case.n_pages)
+    if n_rows:
+        case.tables += [[-1] * case.width for _ in range(n_rows - len(case.tables))]
+    case.device()
+    assert case.run() == case.expected() and case.status.item() == 0
