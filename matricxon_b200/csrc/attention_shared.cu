@@ -304,9 +304,10 @@ shared_simt_kernel(const SharedAttnParams p) {
 }
 
 // The join: a warp a (token, head), four dimensions a lane. A token of no sequence is left alone. So is one whose parts nobody
-// wrote, which is reported: a token that is not its sequence's (by the sequences' starts), whose sequence is in no group, or
-// that does not fit its sequence's narrow tile; with groups whose starts fall, all are. The lists are read before the wait:
-// the kernels before this one have waited for what wrote them, and this one begins after that (from L2, where it is then).
+// wrote, which is reported: a token that is not its sequence's (by the sequences' starts), whose sequence is not in one group
+// (none, or groups that overlap), or that does not fit its sequence's narrow tile; where groups overlap so far that they have
+// more tokens than there are, some tiles of the shared keys found no block, and all rows are. The lists are read before the
+// wait: the kernels before this one have waited for what wrote them, and this one begins after that (from L2, where it is then).
 constexpr int JOIN_WARPS = 4;
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
@@ -326,8 +327,20 @@ shared_join_kernel(const float* part_o, const float* part_ml, T* out, int out_st
         auto start_of = [&](int g) { return min(max(__ldcg(shared.first + g), 0), shared.n_seqs); };
         bool rises = true;
         for (int g = threadIdx.x; g < shared.n_groups; g += JOIN_WARPS * 32) rises = rises && start_of(g) <= start_of(g + 1);
-        written = written && seq >= start_of(0) && seq < start_of(shared.n_groups);
-        written = __syncthreads_and(rises) && written;
+        if (__syncthreads_and(rises)) {
+            written = written && seq >= start_of(0) && seq < start_of(shared.n_groups);
+        } else {
+            // groups that overlap, or a list that is filled up with anything that gives no group
+            unsigned groups = 0, tokens = 0;           // (a lane's tokens stop counting where they are too many)
+            for (int g = lane; g < shared.n_groups; g += 32) {
+                const int first = start_of(g), end = start_of(g + 1);
+                if (first >= end) continue;
+                groups += seq >= first && seq < end;
+                tokens = min(tokens + max(min(__ldcg(cu_q + end), shared.n_tokens) - max(__ldcg(cu_q + first), 0), 0), 0x7fffffffu);
+            }
+            const long long all = (long long)__reduce_add_sync(0xffffffffu, tokens & 0xffffu) + ((long long)__reduce_add_sync(0xffffffffu, tokens >> 16) << 16);
+            written = written && __reduce_add_sync(0xffffffffu, groups) == 1u && all <= shared.n_tokens;
+        }
     }
     pdl_wait();
     if (pair >= n_pairs) return;

@@ -716,8 +716,8 @@ def paged_attention_shared(q: torch.Tensor, q_stride: int, cache: torch.Tensor, 
     be in its table while any sequence sees those keys (otherwise the status word is set). ``q``, ``out``, ``window``, ``softcap`` and ``sink`` as in ``paged_attention``;
     sequence s brings rows ``cu_q[s] .. cu_q[s + 1] - 1``, row i of it at position ``context_lens[s] + i``, which
     ``positions`` and ``tok_seq`` repeat row by row. Rows from ``cu_q[-1]`` on are left alone. So are rows whose ``tok_seq`` is
-    not their sequence, and rows of sequences that no group holds; they set the status word (sequences without tokens need no
-    group).
+    not their sequence, and rows of sequences that no group or more than one holds; they set the status word (sequences without
+    tokens need no group, and a list may be filled up with starts that give none).
 
     ``max_q_len``: no sequence brings more tokens, and all together at most ``n_tokens`` (otherwise the status word is set, and
     what does not fit is left out). ``max_shared_len``,

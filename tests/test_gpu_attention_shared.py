@@ -518,3 +518,28 @@ def test_rows_that_lie_in_one_another_or_too_far_apart_are_refused():
     with pytest.raises(KernelLibraryError):
         one.run(out=torch.zeros(width, dtype=BF16, device=DEV).as_strided((1, width), (1 << 31, 1)))
     close(one, one.run(out=torch.zeros(width, dtype=BF16, device=DEV).as_strided((1, width), (1, 1))))     # one row lies in no other
+
+
+@pytest.mark.parametrize("shape", [SHAPES[0], SHAPES[5], SHAPES[10]], ids=str)
+@pytest.mark.parametrize("first,lost", [([0, 2, 4, 0, 0], ()), ([0, 2, 4, 4, 4, 4], ()), ([0] * 40 + [2] + [4] * 40, ()), ([0, 0, 2, 4, 1, 0], ()),
+                                        ([0, 3, 2, 4], (0, 1, 2, 3)), ([0, 1, 0, 1, 4], (0, 1, 2, 3))], ids=str)
+def test_lists_of_groups_that_are_filled_up(shape, first, lost):
+    """Places without a group behind, between and before the groups; groups that overlap."""
+    step = Step([(64, [(30, 1), (9, 2), (0, 1), (5, 1)])], *shape, seed=3)
+    step.d["first"] = ints(first)
+    if lost:
+        out = step.run(scratch=torch.full((1 << 23,), 1e6, device=DEV))
+        assert step.d["status"].item() == 16 and torch.isnan(out).all()
+    else:
+        close(step, step.run(scratch=torch.full((1 << 23,), 1e6, device=DEV)))
+
+
+@pytest.mark.parametrize("shape", [SHAPES[0], SHAPES[5], SHAPES[10]], ids=str)
+def test_overlapping_groups_beside_sequences_of_none(shape):
+    """As many tokens in groups as there are, but one sequence in two of them and one in none."""
+    step = Step([(64, [(30, 1), (9, 1), (0, 1), (5, 1)])], *shape, seed=3)
+    step.d["first"] = ints([0, 2, 1, 3])
+    out = step.run(scratch=torch.full((1 << 23,), 1e6, device=DEV))
+    assert step.d["status"].item() == 16 and torch.isnan(out[[1, 3]]).all()
+    ref, bound = step.plain()
+    assert ((out[[0, 2]].double().cpu() - ref[[0, 2]]).abs() <= bound[[0, 2]]).all()
